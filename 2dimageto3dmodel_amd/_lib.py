@@ -9,6 +9,7 @@ EXACT_LIB = "libm355_exact.so"
 LIB_PATH = os.path.join(_HERE, "lib", os.environ.get("M355_LIB", EXACT_LIB if os.environ.get("M355_EXACT") == "1" else "libm355.so"))
 
 c_int, c_float, c_void_p, c_size_t = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+c_longlong, c_double = ctypes.c_longlong, ctypes.c_double
 
 
 class M355Error(RuntimeError):
@@ -142,6 +143,13 @@ SIGNATURES = {
     "m355_ipc_close": (c_int, [_P]),
     "m355_ipc_free": (c_int, [_P]),
     "m355_ipc_channels": (c_int, []),
+    "m355_group_norm_ws_bytes": (c_size_t, [c_longlong, c_longlong, c_int, c_int, c_int, c_int]),
+    "m355_group_norm_fwd": (c_int, [_P, _P, _P, c_longlong, c_float, _P, c_int, _P, _P, _P, _P, c_longlong, c_longlong, c_int, c_int,
+                                    c_float, c_int, c_float, c_float, c_int, _P]),
+    "m355_group_norm_bwd": (c_int, [_P, _P, _P, _P, c_longlong, c_float, _P, _P, _P, _P, _P, c_int, _P, c_int, _P, c_longlong,
+                                    c_longlong, c_int, c_int, c_int, c_float, c_int, _P]),
+    "m355_grad_clip_ws_bytes": (c_size_t, [c_int]),
+    "m355_grad_clip": (c_int, [_P, _P, _P, _P, c_int, c_double, c_double, _P, _P, _P]),
     "m355_ipc_allreduce": (c_int, [_P, c_int, _P, c_int, c_int, c_int, _P, c_int, _P]),
 }
 

@@ -1,0 +1,91 @@
+"""CPU: what group norm and gradient clipping refuse -- in Python and at the C entry points (which check before they launch)."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_cpu_tensors_are_refused(pkg):
+    x = torch.zeros(2, 4, 4, 8)
+    with pytest.raises(pkg._lib.M355Error):
+        pkg.group_norm_act(x, 2)
+    with pytest.raises(pkg._lib.M355Error):
+        pkg.group_norm_act([1.0], 2)
+    with pytest.raises(pkg._lib.M355Error):
+        pkg.GroupNormAct2d(32)(x)
+    for f in (pkg.grad_norm, lambda t: pkg.clip_grads_(t, 1.0)):
+        with pytest.raises(pkg._lib.M355Error):
+            f([x])
+        with pytest.raises(ValueError):
+            f([])
+    p = torch.nn.Parameter(torch.zeros(3))
+    assert float(pkg.clip_grad_norm_([p], 1.0)) == 0.0 and float(pkg.clip_grad_norm_([], 1.0)) == 0.0
+    with pytest.raises(ValueError):
+        pkg.clip_grad_norm_([p], -1.0)
+    p.grad = torch.ones(3)
+    with pytest.raises(pkg._lib.M355Error):
+        pkg.clip_grad_norm_([p], 1.0)
+    with pytest.raises(ValueError):
+        pkg.GroupNorm2d(48, 32)
+    with pytest.raises(ValueError):
+        pkg.GroupNormAct2d(48, 0)
+
+
+FAKE = ctypes.c_void_p(0x10000)     # device pointers are only looked at
+
+
+def _fwd(L, n=2, hw=16, c=8, g=2, dtype=2, act=0, res=None, res_w=0, x=FAKE, y=ctypes.c_void_p(0x20000), ws=FAKE):
+    return L.m355_group_norm_fwd(x, None, None, 0, 0.0, res, res_w, y, FAKE, FAKE, ws, n, hw, c, g, 1e-5, act, 0.2, 1.0, dtype, None)
+
+
+def _bwd(L, n=2, hw=16, c=8, g=2, dtype=2, act=0, dres=None, res_w=0, dy=FAKE, dx=ctypes.c_void_p(0x20000)):
+    return L.m355_group_norm_bwd(dy, ctypes.c_void_p(0x30000), None, None, 0, 0.0, FAKE, FAKE, dx, None, None, 0, dres, res_w, FAKE, n, hw, c,
+                                 g, act, 0.2, dtype, None)
+
+
+def test_group_norm_entry_points_check_their_arguments(pkg):
+    L = pkg._lib.lib()
+    for kw in (dict(n=-1), dict(hw=-1), dict(c=0), dict(g=0), dict(g=3), dict(dtype=3), dict(dtype=-1), dict(act=2), dict(n=1 << 31),
+               dict(hw=1 << 40)):
+        assert _fwd(L, **kw) == -1 and L.m355_last_error()
+        assert _bwd(L, **kw) == -1 and L.m355_last_error()
+    assert _fwd(L, x=None) == -1 and b"null" in L.m355_last_error()
+    assert _fwd(L, ws=None) == -1 and _fwd(L, y=FAKE) == -1
+    assert _fwd(L, res=FAKE, res_w=3) == -1 and _fwd(L, res=FAKE, res_w=-2) == -1 and _fwd(L, res=None, res_w=4) == -1
+    assert _fwd(L, res=FAKE, res_w=16, hw=16) == -1                    # one row: no half height
+    assert _bwd(L, dres=FAKE, res_w=0) == -1 and _bwd(L, dres=FAKE, res_w=16, hw=16) == -1
+    assert _bwd(L, dy=None) == -1 and _bwd(L, dx=FAKE) == -1
+    # a group wider than a workgroup: 257 odd channels, 4096 of a vector of eight
+    for c, g, dtype in ((257, 1, 2), (771, 3, 0), (4096, 1, 2), (2056, 1, 2)):
+        assert _fwd(L, c=c, g=g, dtype=dtype) == -2 and _bwd(L, c=c, g=g, dtype=dtype) == -2
+    # nothing to do is no error, and launches nothing
+    assert _fwd(L, n=0) == 0 and _fwd(L, hw=0) == 0 and _bwd(L, n=0) == 0 and _bwd(L, hw=0) == 0
+    assert L.m355_group_norm_ws_bytes(2, 16, 8, 3, 2, 0) == 0
+    small, back = L.m355_group_norm_ws_bytes(2, 16, 8, 2, 2, 0), L.m355_group_norm_ws_bytes(2, 16, 8, 2, 2, 1)
+    assert small >= 2 * 2 * 8 and back >= small + 2 * 2 * 8 * 4
+
+
+def _clip(L, ins, outs, numel, dtype, scale=1.0, max_norm=1.0, norm=FAKE, ws=FAKE):
+    n = len(numel)
+    arr = (lambda v: None if v is None else (ctypes.c_void_p * n)(*v))
+    return L.m355_grad_clip(arr(ins), arr(outs), (ctypes.c_longlong * n)(*numel), (ctypes.c_int * n)(*dtype), n, scale, max_norm, norm, ws, None)
+
+
+def test_clip_entry_point_checks_its_arguments(pkg):
+    L = pkg._lib.lib()
+    a, b = 0x100000, 0x200000
+    ok = dict(numel=[100, 100], dtype=[0, 0])
+    for kw in (dict(scale=float("nan")), dict(scale=float("inf")), dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(norm=None),
+               dict(ws=None)):
+        assert _clip(L, [a, b], [a, b], **ok, **kw) == -1 and L.m355_last_error()
+    assert _clip(L, [a, b], [a, b], [100, -1], [0, 0]) == -1 and _clip(L, [a, b], [a, b], [100, 1 << 41], [0, 0]) == -1
+    assert _clip(L, [a, b], [a, b], [100, 100], [0, 3]) == -1
+    assert _clip(L, [a, None], [a, b], **ok) == -1 and _clip(L, [a, b], [a, None], **ok) == -1
+    assert _clip(L, [a, b + 2], [a, b + 2], **ok) == -1 and _clip(L, [a, b], [a, b + 1], [100, 100], [0, 1]) == -1
+    # memory that two tensors share: 100 floats are 400 bytes
+    shared = [([a, a], [a, a]), ([a, a + 396], [a, a + 396]), ([a, b], [a, a + 4]), ([a, b], [b + 0x1000, a]), ([a, b], [a + 8, b]),
+              ([a, b], [b, a]), ([a, b], [b + 0x1000, b + 0x1000])]
+    for ins, outs in shared:
+        assert _clip(L, ins, outs, **ok) == -1 and b"shares memory" in L.m355_last_error(), (ins, outs)
+    assert L.m355_grad_clip_ws_bytes(-1) == 0
+    assert L.m355_grad_clip_ws_bytes(0) == L.m355_grad_clip_ws_bytes(112) == 8 * 1024 and L.m355_grad_clip_ws_bytes(113) == 2 * 8 * 1024
