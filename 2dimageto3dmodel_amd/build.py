@@ -40,6 +40,9 @@ SOURCES = [
     ("gan_io.hip", []),
     ("ipc_exchange.hip", []),
     ("group_norm.hip", NO_PK),
+    ("group_norm_f32.hip", NO_PK),
+    ("group_norm_f16.hip", NO_PK),
+    ("group_norm_bf16.hip", NO_PK),
     ("grad_clip.hip", NO_PK),
     ("mesh_deform.hip", STRICT),
     ("dibr_raster.hip", STRICT),

@@ -1,0 +1,6 @@
+// The group norm kernels of one element type (group_norm.h).
+#include <type_traits>
+
+#define M355_GN_T _Float16
+#define M355_GN_RUN run_f16
+#include "group_norm_types.h"

@@ -97,15 +97,15 @@ class _GroupNormAct(torch.autograd.Function):
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty(weight.shape, dtype=torch.float32, device=dev) if need_w else None
         db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if need_b else None
-        dres, half = None, False
+        half = res_shape is not None and res_shape != tuple(x.shape)
+        dres = None
         if need_r:
-            half = res_shape != tuple(x.shape)
             dres = torch.empty(res_shape, dtype=x.dtype, device=dev) if half else dy
         if x.numel() == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-        elif need_x or need_w or need_b or half:
+        elif need_x or need_w or need_b or (half and need_r):
             one = weight if weight is not None else bias
             per_sample = one is not None and one.dim() == 2
             with _on(x):

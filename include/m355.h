@@ -569,8 +569,8 @@ int m355_ipc_allreduce(float *inout, int n, void *const *regions /*[world], host
  *      through the nearest x2 upsample (res_w = full width; even height and width).  mean, rstd [N][G] are written for the backward.
  *      ws >= m355_group_norm_ws_bytes(.., 0) bytes, 16-byte aligned; 0 = bad sizes.  A group of more channels than 256 vectors of at most
  *      16 bytes hold is M355_ERR_UNSUPPORTED.  Nothing is launched for N == 0 or HW == 0.
- *      _bwd: dy -> dx (nullable), dw / db (nullable; per_sample: [N][C], else [C] summed over the samples; overwritten), dres (nullable:
- *      2 x 2 sums of dy, [N][H/2][res_w/2][C]).  The derivative of out_slope is the caller's (as m355_affine_act_fwd). */
+ *      _bwd: dy -> dx (nullable), dw / db (nullable; per_sample: [N][C], else [C] summed over the samples; overwritten), res_w as
+ *      in the forward, dres (nullable: 2 x 2 sums of dy, [N][H/2][res_w/2][C]).  The derivative of out_slope is the caller's (as m355_affine_act_fwd). */
 size_t m355_group_norm_ws_bytes(long long N, long long HW, int C, int G, int dtype, int backward);
 int m355_group_norm_fwd(const void *x, const float *w, const float *b, long long aff_stride, float w_off, const void *res, int res_w,
                         void *y, float *mean, float *rstd, void *ws, long long N, long long HW, int C, int G, float eps, int act,
