@@ -143,11 +143,9 @@ SIGNATURES = {
     "m355_ipc_close": (c_int, [_P]),
     "m355_ipc_free": (c_int, [_P]),
     "m355_ipc_channels": (c_int, []),
-    "m355_group_norm_ws_bytes": (c_size_t, [c_longlong, c_longlong, c_int, c_int, c_int, c_int]),
-    "m355_group_norm_fwd": (c_int, [_P, _P, _P, c_longlong, c_float, _P, c_int, _P, _P, _P, _P, c_longlong, c_longlong, c_int, c_int,
-                                    c_float, c_int, c_float, c_float, c_int, _P]),
-    "m355_group_norm_bwd": (c_int, [_P, _P, _P, _P, c_longlong, c_float, _P, _P, _P, _P, _P, c_int, _P, c_int, _P, c_longlong,
-                                    c_longlong, c_int, c_int, c_int, c_float, c_int, _P]),
+    "m355_group_norm_ws_bytes": (c_size_t, [_P, c_int]),
+    "m355_group_norm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "m355_group_norm_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "m355_grad_clip_ws_bytes": (c_size_t, [c_int]),
     "m355_grad_clip": (c_int, [_P, _P, _P, _P, c_int, c_double, c_double, _P, _P, _P]),
     "m355_ipc_allreduce": (c_int, [_P, c_int, _P, c_int, c_int, c_int, _P, c_int, _P]),
@@ -168,6 +166,13 @@ class ConvPlan(ctypes.Structure):
                 ("fwd_ws_stats_rows", c_int), ("wgrad_fuses_dbias", c_int),
                 ("fwd_ws_bytes", c_size_t), ("dgrad_ws_bytes", c_size_t), ("wgrad_ws_bytes", c_size_t),
                 ("wgrad_det_ws_bytes", c_size_t), ("exec_ratio", ctypes.c_double), ("w_dgrad_row_elems", c_int), ("wgrad_ws_ordered", c_int)]
+
+
+class GnDesc(ctypes.Structure):
+    """m355_gn_desc (include/m355.h)"""
+    _fields_ = [(n, c_longlong) for n in ("N", "HW", "aff_stride")] + \
+               [(n, c_int) for n in ("C", "G", "dtype", "act", "res_w", "per_sample")] + \
+               [(n, c_float) for n in ("eps", "slope", "out_slope", "w_off")]
 
 
 class SnFinEntry(ctypes.Structure):

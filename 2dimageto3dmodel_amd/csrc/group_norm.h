@@ -19,6 +19,23 @@
 namespace m355 {
 namespace gn {
 
+// division by a number the host knows: exact for dividends below 2^31
+struct Div {
+    unsigned d, mul, shift;
+    __host__ void set(unsigned by)
+    {
+        d = by;
+        mul = shift = 0;
+        if (by > 1) {
+            int l = 0;
+            while ((1ULL << l) < by) ++l;
+            mul = (unsigned)(((1ULL << (31 + l)) / by) + 1);
+            shift = (unsigned)(l - 1);
+        }
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+
 struct Args {
     const void *x, *dy, *res;
     void *y, *dres;               // y: forward's result, backward's dx (NULL: not wanted)
@@ -36,8 +53,9 @@ struct Args {
     int SC, LV, PL, nslab;        // channels of a slab (whole groups, whole vectors), vectors across it, pixel lanes, slabs
     int nblk, gnblk;              // ranges of a sample in this kernel; rows of gpart / cpart a sample
     int act, per_sample, quad, finished;
-    int W2;                       // quad: half the width; h = i / W2 = umulhi(i, magic) >> shift for i < 2^31
-    unsigned magic, shift;
+    int nt;                       // outputs and the second pass's inputs go past the memory-side cache
+    int W2;                       // quad: half the width
+    Div by_w2, by_lv, by_pl, by_nslab, by_nblk, by_d, by_sg;   // sg = D / (channels of a segment)
     float w_off, eps, slope, out_slope;
 };
 
@@ -49,13 +67,25 @@ template <typename T, int V> struct IO {
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = (float)v[j];
     }
-    static __device__ __forceinline__ void store(T *p, const float (&f)[V])
+    // NT: past the memory-side cache
+    template <bool NT> static __device__ __forceinline__ raw load(const T *p)
+    {
+        if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const raw *>(p));
+        else return *reinterpret_cast<const raw *>(p);
+    }
+    static __device__ __forceinline__ raw pack(const float (&f)[V])
     {
         raw v;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = (T)f[j];   // to nearest even, once, from the 32-bit result
-        *reinterpret_cast<raw *>(p) = v;
+        return v;
     }
+    template <bool NT> static __device__ __forceinline__ void put(T *p, const raw &v)
+    {
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<raw *>(p));
+        else *reinterpret_cast<raw *>(p) = v;
+    }
+    template <bool NT> static __device__ __forceinline__ void store(T *p, const float (&f)[V]) { put<NT>(p, pack(f)); }
 };
 
 // the registers of a loaded vector are used again later: keeps the compiler from carrying its 32-bit form (twice the registers) along
@@ -71,36 +101,39 @@ template <typename R> __device__ __forceinline__ void keep(R &v)
     }
 }
 
+constexpr int kT = 256;   // threads of a workgroup
+
 struct Place {   // what a workgroup and a thread of it own
     int n, slab, blk, lv, pl, c0, ng;   // ng: groups of the slab
     bool on;
     long long i0, ni;                   // items
-    __device__ __forceinline__ Place(const Args &a, long long id, int V)
+    __device__ __forceinline__ Place(const Args &a, unsigned id, int V)
     {
-        const unsigned u = (unsigned)id;   // (the grid's work fits 32 bits: checked by the host)
-        blk = (int)(u % (unsigned)a.nblk);
-        const unsigned r = u / (unsigned)a.nblk;
-        slab = (int)(r % (unsigned)a.nslab);
-        n = (int)(r / (unsigned)a.nslab);
-        lv = (int)(threadIdx.x % (unsigned)a.LV);
-        pl = (int)(threadIdx.x / (unsigned)a.LV);
+        const unsigned r = a.by_nblk.of(id);   // (below 2^23: the host's launches)
+        blk = (int)(id - r * (unsigned)a.nblk);
+        n = (int)a.by_nslab.of(r);
+        slab = (int)r - n * a.nslab;
+        pl = (int)a.by_lv.of(threadIdx.x);
+        lv = (int)threadIdx.x - pl * a.LV;
         c0 = slab * a.SC + lv * V;
         on = pl < a.PL && c0 < a.C;
-        ng = min(a.SC, a.C - slab * a.SC) / a.D;
+        ng = (int)a.by_d.of((unsigned)min(a.SC, a.C - slab * a.SC));
         i0 = (long long)blk * a.per;
         ni = min(a.per, a.items - i0);
     }
-    __device__ __forceinline__ int g0(const Args &a) const { return slab * (a.SC / a.D); }
+    __device__ __forceinline__ int g0(const Args &a) const { return slab * (int)a.by_d.of((unsigned)a.SC); }
 };
 
-// row of the 2 x 2 block i < 2^31
-__device__ __forceinline__ unsigned row_of(const Args &a, unsigned i) { return a.W2 == 1 ? i : __umulhi(i, a.magic) >> a.shift; }
+__device__ __forceinline__ int vectors_of(const Args &a, const Place &pc)
+{
+    return pc.on && pc.pl < pc.ni ? (int)a.by_pl.of((unsigned)((int)pc.ni - pc.pl + a.PL - 1)) : 0;   // (a range has fewer than 2^31 items: checked by the host)
+}
 
 // first pixel of item i (quad: the block's top left one; the others are 1, W and W + 1 further)
 __device__ __forceinline__ long long first_pixel(const Args &a, long long i)
 {
     if (!a.quad) return i;
-    const long long h = a.items < (1LL << 31) ? (long long)row_of(a, (unsigned)i) : i / a.W2;
+    const long long h = a.items < (1LL << 31) ? (long long)a.by_w2.of((unsigned)i) : i / a.W2;
     return 2 * (i + h * a.W2);
 }
 
@@ -108,17 +141,12 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 
 // ---- sums over a workgroup's threads by group.  sh: [rows][stride], row = pixel lane, sg columns a group; odd strides keep the
 // lanes of a group off each other's banks.  tpg (a power of two, at most 64) neighbouring threads add up a group, its first one has f.
-__device__ __forceinline__ int threads_per_group(int nt, int ng)
+template <typename F> __device__ __forceinline__ void by_group(int ng, F f)
 {
-    int t = 64;
-    while (t > 1 && t * ng > nt) t >>= 1;
-    return t;
-}
-
-template <typename F> __device__ __forceinline__ void by_group(int nt, int ng, F f)
-{
-    const int tpg = threads_per_group(nt, ng), k = (int)threadIdx.x & (tpg - 1);
-    for (int g = (int)threadIdx.x / tpg; g < ng; g += nt / tpg) f(g, k, tpg);
+    int l = 6;
+    while (l > 0 && (ng << l) > kT) --l;
+    const int k = (int)threadIdx.x & ((1 << l) - 1);
+    for (int g = (int)threadIdx.x >> l; g < ng; g += kT >> l) f(g, k, 1 << l);
 }
 
 __device__ __forceinline__ float lanes_sum(float v, int tpg)
@@ -127,17 +155,13 @@ __device__ __forceinline__ float lanes_sum(float v, int tpg)
     return v;
 }
 
-__device__ __forceinline__ float columns_sum(const float *sh, int stride, int rows, int sg, int g, int k, int tpg)
+__device__ __forceinline__ float columns_sum(const float *sh, int stride, int rows, const Div &by_sg, int g, int k, int tpg)
 {
     float s = 0.0f;
-    const int total = rows * sg;
-    if (sg == 1) {
-        for (int e = k; e < total; e += tpg) s += sh[e * stride + g];
-    } else {
-        for (int e = k; e < total; e += tpg) {
-            const int r = (unsigned)e / (unsigned)sg;
-            s += sh[r * stride + g * sg + e - r * sg];
-        }
+    const int sg = (int)by_sg.d, total = rows * sg;
+    for (int e = k; e < total; e += tpg) {
+        const int r = (int)by_sg.of((unsigned)e);
+        s += sh[r * stride + g * sg + e - r * sg];
     }
     return lanes_sum(s, tpg);
 }
@@ -145,11 +169,16 @@ __device__ __forceinline__ float columns_sum(const float *sh, int stride, int ro
 // the affine of the thread's channels
 template <int V> __device__ __forceinline__ void affine(const Args &a, const Place &pc, float (&w)[V], float (&b)[V])
 {
+    typedef float row __attribute__((ext_vector_type(V), aligned(4)));   // (the rows may start at any float)
     const long long i = (long long)pc.n * a.aff_stride + pc.c0;
+    row wv = {}, bv = {};
+    if (pc.on && a.w) wv = *reinterpret_cast<const row *>(a.w + i);
+    if (pc.on && a.b) bv = *reinterpret_cast<const row *>(a.b + i);
+    const float off = a.w ? a.w_off : 1.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        w[j] = (pc.on && a.w) ? a.w[i + j] + a.w_off : 1.0f;
-        b[j] = (pc.on && a.b) ? a.b[i + j] : 0.0f;
+        w[j] = wv[j] + off;
+        b[j] = bv[j];
     }
 }
 
@@ -196,13 +225,13 @@ template <int V, int A> struct Stat {
     }
 };
 
-// joins the threads' statistics: s_mean / s_m2 [groups of the slab].  `pixels`: this thread's, `all`: the workgroup's.  sh: NT * (A + 1)
-template <int NT, int V, int A>
+// joins the threads' statistics: s_mean / s_m2 [groups of the slab].  `pixels`: this thread's, `all`: the workgroup's.  sh: kT * (A + 1)
+template <int V, int A>
 __device__ __forceinline__ void join_threads(const Args &a, const Place &pc, const Stat<V, A> &st, float pixels, float all, float *sh,
                                              float *s_mean, float *s_m2)
 {
     constexpr int S = V / A;
-    const int sg = a.D / S, stride = (a.LV * A) | 1;
+    const int stride = (a.LV * A) | 1;
     const float inv = 1.0f / (all * (float)a.D);
     float *mine = sh + pc.pl * stride + pc.lv * A;
     if (pc.pl < a.PL) {
@@ -210,29 +239,29 @@ __device__ __forceinline__ void join_threads(const Args &a, const Place &pc, con
         for (int k = 0; k < A; ++k) mine[k] = pc.on ? pixels * S * st.K[k] : 0.0f;
     }
     __syncthreads();
-    by_group(NT, pc.ng, [&](int g, int k, int tpg) {
-        const float v = columns_sum(sh, stride, a.PL, sg, g, k, tpg);
+    by_group(pc.ng, [&](int g, int k, int tpg) {
+        const float v = columns_sum(sh, stride, a.PL, a.by_sg, g, k, tpg);
         if (k == 0) s_mean[g] = v * inv;
     });
     __syncthreads();
     if (pc.on) {
 #pragma unroll
         for (int k = 0; k < A; ++k) {
-            const float d = st.K[k] - s_mean[(pc.lv * A + k) / sg];
+            const float d = st.K[k] - s_mean[a.by_sg.of((unsigned)(pc.lv * A + k))];
             mine[k] = st.q[k] + pixels * S * d * d;
         }
     }
     __syncthreads();
-    by_group(NT, pc.ng, [&](int g, int k, int tpg) {
-        const float v = columns_sum(sh, stride, a.PL, sg, g, k, tpg);
+    by_group(pc.ng, [&](int g, int k, int tpg) {
+        const float v = columns_sum(sh, stride, a.PL, a.by_sg, g, k, tpg);
         if (k == 0) s_m2[g] = v;
     });
 }
 
-// y of one vector at pixel offset `o` (elements from the sample's channel c0)
-template <typename T, int V, int A, int ACT>
+// y of one vector; `add`: plus the residual's vector
+template <typename T, int V, int A, int ACT, bool NT>
 __device__ __forceinline__ void finish_store(const Args &a, const float (&f)[V], const float (&mu)[A], const float (&k)[V], const float (&b)[V],
-                                             const T *res, T *y)
+                                             bool add, const typename IO<T, V>::raw &res, T *y)
 {
     constexpr int S = V / A;
     float z[V];
@@ -245,9 +274,9 @@ __device__ __forceinline__ void finish_store(const Args &a, const float (&f)[V],
 #pragma unroll
         for (int j = 0; j < V; ++j) z[j] = z[j] * sigmoid(z[j]);
     }
-    if (res) {
+    if (add) {
         float r[V];
-        IO<T, V>::open(IO<T, V>::load(res), r);
+        IO<T, V>::open(res, r);
 #pragma unroll
         for (int j = 0; j < V; ++j) z[j] += r[j];
     }
@@ -255,7 +284,7 @@ __device__ __forceinline__ void finish_store(const Args &a, const float (&f)[V],
 #pragma unroll
         for (int j = 0; j < V; ++j) z[j] = z[j] >= 0.0f ? z[j] : z[j] * a.out_slope;
     }
-    IO<T, V>::store(y, z);
+    IO<T, V>::template store<NT>(y, z);
 }
 
 // xc = x - mean and dz of one vector.  z is computed as the forward computes it: the sign a LeakyReLU's gradient goes by is the forward's
@@ -278,8 +307,6 @@ __device__ __forceinline__ void grad_of(const Args &a, const float (&f)[V], cons
     }
 }
 
-constexpr int kT = 256;   // threads of the two-pass kernels
-
 // ---- forward, first of two passes: gpart[n][blk][g] = (mean, M2) of the workgroup's pixels
 template <typename T, int V, int A> __global__ __launch_bounds__(kT) void k_gn_stats(const Args a)
 {
@@ -290,7 +317,7 @@ template <typename T, int V, int A> __global__ __launch_bounds__(kT) void k_gn_s
     Stat<V, A> st;
     st.start();
     const int ni = (int)pc.ni;   // (a range has fewer than 2^31 pixels: checked by the host)
-    const int mine = pc.on ? max(0, (ni - pc.pl + a.PL - 1) / a.PL) : 0;
+    const int mine = vectors_of(a, pc);
     if (mine > 0) {
         const size_t step = (size_t)a.PL * a.C;
         const T *p = x + (size_t)pc.pl * a.C;
@@ -325,25 +352,44 @@ template <typename T, int V, int A> __global__ __launch_bounds__(kT) void k_gn_s
         }
         st.close((float)mine);
     }
-    join_threads<kT, V, A>(a, pc, st, (float)mine, (float)ni, sh, s_mean, s_m2);
+    join_threads<V, A>(a, pc, st, (float)mine, (float)ni, sh, s_mean, s_m2);
     __syncthreads();
     float2 *out = a.gpart + ((size_t)pc.n * a.gnblk + pc.blk) * a.G + pc.g0(a);
     for (int g = threadIdx.x; g < pc.ng; g += kT) out[g] = make_float2(s_mean[g], s_m2[g]);
 }
 
-// mean and rstd of a group from its ranges' parts, by tpg lanes
+// mean and rstd of a group from its ranges' parts, by tpg lanes: the parts of up to kBatch ranges a lane are loaded at once
+constexpr int kBatch = 4;
 __device__ __forceinline__ void join_ranges(const Args &a, int n, int g, int k, int tpg, float &mu, float &rs)
 {
     const float2 *p = a.gpart + (size_t)n * a.gnblk * a.G + g;
-    const float m = (float)((double)a.hw * a.D);
+    const float m = (float)((double)a.hw * a.D), full = (float)a.gper * a.D;
+    const float tail = (float)(a.hw - (long long)(a.gnblk - 1) * a.gper) * a.D;   // values of the last range
     float s = 0.0f, q = 0.0f;
-    for (int i = k; i < a.gnblk; i += tpg)
-        s += p[(size_t)i * a.G].x * ((float)min(a.gper, a.hw - (long long)i * a.gper) * a.D);
-    mu = lanes_sum(s, tpg) / m;
-    for (int i = k; i < a.gnblk; i += tpg) {
-        const float2 v = p[(size_t)i * a.G];
-        const float d = v.x - mu;
-        q += v.y + d * d * ((float)min(a.gper, a.hw - (long long)i * a.gper) * a.D);
+    if (a.gnblk <= kBatch * tpg) {
+        float2 v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = k + u * tpg;
+            v[u] = i < a.gnblk ? p[(size_t)i * a.G] : make_float2(0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) s += v[u].x * (k + u * tpg < a.gnblk - 1 ? full : tail);
+        mu = lanes_sum(s, tpg) / m;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = k + u * tpg;
+            const float d = v[u].x - mu;
+            if (i < a.gnblk) q += v[u].y + d * d * (i < a.gnblk - 1 ? full : tail);
+        }
+    } else {
+        for (int i = k; i < a.gnblk; i += tpg) s += p[(size_t)i * a.G].x * (i < a.gnblk - 1 ? full : tail);
+        mu = lanes_sum(s, tpg) / m;
+        for (int i = k; i < a.gnblk; i += tpg) {
+            const float2 v = p[(size_t)i * a.G];
+            const float d = v.x - mu;
+            q += v.y + d * d * (i < a.gnblk - 1 ? full : tail);
+        }
     }
     rs = 1.0f / sqrtf(lanes_sum(q, tpg) / m + a.eps);
 }
@@ -362,89 +408,126 @@ static __global__ __launch_bounds__(kT) void k_gn_finish(const Args a)
     }
 }
 
-// ---- forward, second pass
-template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) void k_gn_apply(const Args a)
+// A walk over a thread's vectors in steps of R, the next step's loads in flight while f works on this one and stores: a wait for a load also
+// waits for the stores issued before it (one counter, in order), and a loop that loads behind its stores pays their way to memory each
+// time round.  start() issues the first loads; run() walks.
+template <int R, typename Raw, int K> struct Ahead {
+    Raw v[K][R];
+    template <typename G> __device__ __forceinline__ void start(int mine, G get)
+    {
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+            if (u < mine) get(v, u, u);
+    }
+    template <typename G, typename F> __device__ __forceinline__ void run(int mine, G get, F f)
+    {
+        for (int i = 0; i < mine; i += R) {
+            Raw n[K][R];
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+                if (i + R + u < mine) get(n, u, i + R + u);
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+                if (i + u < mine) f(v, u, i + u);
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int k = 0; k < K; ++k) v[k][u] = n[k][u];
+        }
+    }
+};
+
+// mean and rstd of the slab's groups
+__device__ __forceinline__ void slab_stats(const Args &a, const Place &pc, float *s_mean, float *s_rstd)
 {
-    constexpr int S = V / A;
-    __shared__ float s_mean[kT * A], s_rstd[kT * A];
-    const Place pc(a, blockIdx.x, V);
     const int g0 = pc.g0(a);
     if (a.finished) {
         for (int g = threadIdx.x; g < pc.ng; g += kT) {
             s_mean[g] = a.mean[(size_t)pc.n * a.G + g0 + g];
             s_rstd[g] = a.rstd[(size_t)pc.n * a.G + g0 + g];
         }
-    } else {
-        by_group(kT, pc.ng, [&](int g, int k, int tpg) {
-            float mu, rs;
-            join_ranges(a, pc.n, g0 + g, k, tpg, mu, rs);
-            if (k == 0) {
-                s_mean[g] = mu;
-                s_rstd[g] = rs;
-                if (pc.blk == 0) {
-                    a.mean[(size_t)pc.n * a.G + g0 + g] = mu;
-                    a.rstd[(size_t)pc.n * a.G + g0 + g] = rs;
-                }
+        return;
+    }
+    by_group(pc.ng, [&](int g, int k, int tpg) {
+        float mu, rs;
+        join_ranges(a, pc.n, g0 + g, k, tpg, mu, rs);
+        if (k == 0) {
+            s_mean[g] = mu;
+            s_rstd[g] = rs;
+            if (pc.blk == 0) {
+                a.mean[(size_t)pc.n * a.G + g0 + g] = mu;
+                a.rstd[(size_t)pc.n * a.G + g0 + g] = rs;
             }
-        });
-    }
-    float k[V], b[V], mu[A];
-    affine<V>(a, pc, k, b);
-    __syncthreads();
-    if (!pc.on) return;
-    const int sg = a.D / S;
-#pragma unroll
-    for (int j = 0; j < A; ++j) {
-        const int g = (pc.lv * A + j) / sg;
-        mu[j] = s_mean[g];
-#pragma unroll
-        for (int u = 0; u < S; ++u) k[j * S + u] *= s_rstd[g];
-    }
-    const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0;
+        }
+    });
+}
+
+// ---- forward, second pass
+template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds__(kT) void k_gn_apply(const Args a)
+{
+    constexpr int S = V / A;
+    typedef typename IO<T, V>::raw raw;
+    __shared__ float s_mean[kT * A], s_rstd[kT * A];
+    const Place pc(a, blockIdx.x, V);
+    const int mine = vectors_of(a, pc);
+    const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0, step = (size_t)a.PL * a.C;
     const T *x = (const T *)a.x + base;
     T *y = (T *)a.y + base;
+    float k[V], b[V], mu[A];
+    auto coefficients = [&]() {
+        affine<V>(a, pc, k, b);
+        slab_stats(a, pc, s_mean, s_rstd);
+        __syncthreads();
+        if (!pc.on) return;
+#pragma unroll
+        for (int j = 0; j < A; ++j) {
+            const int g = (int)a.by_sg.of((unsigned)(pc.lv * A + j));
+            mu[j] = s_mean[g];
+#pragma unroll
+            for (int u = 0; u < S; ++u) k[j * S + u] *= s_rstd[g];
+        }
+    };
     if (a.quad) {   // the residual is read once for its four pixels
         const T *res = (const T *)a.res + (size_t)pc.n * a.items * a.C + pc.c0;
         const size_t row = (size_t)2 * a.W2 * a.C;
-        for (long long i = pc.i0 + pc.pl; i < pc.i0 + pc.ni; i += a.PL) {
-            const size_t o = (size_t)first_pixel(a, i) * a.C;
-            const typename IO<T, V>::raw v0 = IO<T, V>::load(x + o), v1 = IO<T, V>::load(x + o + a.C), v2 = IO<T, V>::load(x + o + row),
-                                         v3 = IO<T, V>::load(x + o + row + a.C);
-            const T *r = res + (size_t)i * a.C;
-            float f[V];
-            IO<T, V>::open(v0, f);
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, r, y + o);
-            IO<T, V>::open(v1, f);
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, r, y + o + a.C);
-            IO<T, V>::open(v2, f);
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, r, y + o + row);
-            IO<T, V>::open(v3, f);
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, r, y + o + row + a.C);
-        }
+        const long long i0 = pc.i0 + pc.pl;
+        Ahead<1, raw, 5> w;
+        auto get = [&](raw (&v)[5][1], int, int i) {
+            const long long q = i0 + (long long)i * a.PL;
+            const T *p = x + (size_t)first_pixel(a, q) * a.C;
+            v[0][0] = IO<T, V>::template load<NT>(p);
+            v[1][0] = IO<T, V>::template load<NT>(p + a.C);
+            v[2][0] = IO<T, V>::template load<NT>(p + row);
+            v[3][0] = IO<T, V>::template load<NT>(p + row + a.C);
+            v[4][0] = IO<T, V>::template load<NT>(res + (size_t)q * a.C);
+        };
+        w.start(mine, get);
+        coefficients();
+        w.run(mine, get, [&](raw (&v)[5][1], int, int i) {
+            T *p = y + (size_t)first_pixel(a, i0 + (long long)i * a.PL) * a.C;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float f[V];
+                IO<T, V>::open(v[u][0], f);
+                finish_store<T, V, A, ACT, NT>(a, f, mu, k, b, true, v[4][0], p + (u & 1) * a.C + (u >> 1) * row);
+            }
+        });
         return;
     }
-    constexpr int R = 4;
     const T *res = a.res ? (const T *)a.res + base : nullptr;
-    const size_t step = (size_t)a.PL * a.C;
-    const int mine = max(0, ((int)pc.ni - pc.pl + a.PL - 1) / a.PL);
-    size_t o = (size_t)(pc.i0 + pc.pl) * a.C;
-    int i = 0;
-    for (; i + R <= mine; i += R, o += R * step) {
-        typename IO<T, V>::raw v[R];
-#pragma unroll
-        for (int u = 0; u < R; ++u) v[u] = IO<T, V>::load(x + o + u * step);
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            float f[V];
-            IO<T, V>::open(v[u], f);
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, res ? res + o + u * step : nullptr, y + o + u * step);
-        }
-    }
-    for (; i < mine; ++i, o += step) {
+    const size_t o = (size_t)(pc.i0 + pc.pl) * a.C;
+    Ahead<2, raw, 2> w;
+    auto get = [&](raw (&v)[2][2], int u, int i) {
+        v[0][u] = IO<T, V>::template load<NT>(x + o + i * step);
+        if (res) v[1][u] = IO<T, V>::template load<NT>(res + o + i * step);
+    };
+    w.start(mine, get);
+    coefficients();
+    w.run(mine, get, [&](raw (&v)[2][2], int u, int i) {
         float f[V];
-        IO<T, V>::open(IO<T, V>::load(x + o), f);
-        finish_store<T, V, A, ACT>(a, f, mu, k, b, res ? res + o : nullptr, y + o);
-    }
+        IO<T, V>::open(v[0][u], f);
+        finish_store<T, V, A, ACT, NT>(a, f, mu, k, b, res != nullptr, v[1][u], y + o + i * step);
+    });
 }
 
 // statistics and affine of the thread's channels for the backward: k = rstd * w as the forward multiplied it
@@ -455,7 +538,7 @@ __device__ __forceinline__ void saved(const Args &a, const Place &pc, float (&mu
     affine<V>(a, pc, k, b);
 #pragma unroll
     for (int j = 0; j < A; ++j) {
-        const size_t g = (size_t)pc.n * a.G + (pc.on ? (pc.c0 + j * S) / a.D : 0);
+        const size_t g = (size_t)pc.n * a.G + (pc.on ? a.by_d.of((unsigned)(pc.c0 + j * S)) : 0u);
         mu[j] = a.mean[g];
         rs[j] = a.rstd[g];
 #pragma unroll
@@ -464,8 +547,8 @@ __device__ __forceinline__ void saved(const Args &a, const Place &pc, float (&mu
 }
 
 // joins the threads' per-channel sums (t1: dz, t2: dz (x - mean)): cpart row `row` (unless NULL), and per group
-// s1 / s2 [groups of the slab] = sum w dz, sum w dz xhat.  sh1, sh2: NT * (V + 1)
-template <int NT, int V, int A>
+// s1 / s2 [groups of the slab] = sum w dz, sum w dz xhat.  sh1, sh2: kT * (V + 1)
+template <int V, int A>
 __device__ __forceinline__ void join_grads(const Args &a, const Place &pc, const float (&t1)[V], const float (&t2)[V], const float (&rs)[A],
                                            float *sh1, float *sh2, float *s1, float *s2, float *out1, float *out2)
 {
@@ -480,8 +563,9 @@ __device__ __forceinline__ void join_grads(const Args &a, const Place &pc, const
     }
     __syncthreads();
     const int cs = pc.slab * a.SC, nc = pc.ng * a.D;
-    by_group(NT, nc, [&](int c, int k, int tpg) {
+    by_group(nc, [&](int c, int k, int tpg) {
         float u1 = 0.0f, u2 = 0.0f;
+#pragma unroll 2
         for (int r = k; r < a.PL; r += tpg) {
             u1 += sh1[r * stride + c];
             u2 += sh2[r * stride + c];
@@ -497,7 +581,7 @@ __device__ __forceinline__ void join_grads(const Args &a, const Place &pc, const
         }
     });
     __syncthreads();
-    by_group(NT, pc.ng, [&](int g, int k, int tpg) {
+    by_group(pc.ng, [&](int g, int k, int tpg) {
         float u1 = 0.0f, u2 = 0.0f;
         for (int c = k; c < a.D; c += tpg) {
             u1 += sh1[g * a.D + c];
@@ -513,10 +597,10 @@ __device__ __forceinline__ void join_grads(const Args &a, const Place &pc, const
 }
 
 // ---- backward, first pass: per-channel sums of dz and dz xhat, their weighted sums per group; the half-resolution residual's gradient
-template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) void k_gn_bwd_reduce(const Args a)
+template <typename T, int V, int A, int ACT, bool NT>
+__device__ __forceinline__ void grads_of_range(const Args &a, unsigned id, float *sh1, float *sh2, float *s1, float *s2)
 {
-    __shared__ float sh1[kT * (V + 1)], sh2[kT * (V + 1)], s1[kT * A], s2[kT * A];
-    const Place pc(a, blockIdx.x, V);
+    const Place pc(a, id, V);
     const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0;
     const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base;
     float mu[A], rs[A], k[V], b[V], t1[V], t2[V];
@@ -535,7 +619,9 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
     };
     if (pc.on && a.quad) {
         const size_t row = (size_t)2 * a.W2 * a.C;
-        T *dres = (T *)a.dres + (size_t)pc.n * a.items * a.C + pc.c0;
+        T *dres = (T *)a.dres + (size_t)pc.n * a.items * a.C + pc.c0, *last = nullptr;
+        typename IO<T, V>::raw kept = {};   // (stored behind the next loads, as the forward does)
+#pragma unroll 1
         for (long long i = pc.i0 + pc.pl; i < pc.i0 + pc.ni; i += a.PL) {
             const size_t o = (size_t)first_pixel(a, i) * a.C;
             const size_t at[4] = {o, o + a.C, o + row, o + row + a.C};
@@ -545,6 +631,7 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
                 vx[u] = IO<T, V>::load(x + at[u]);
                 vd[u] = IO<T, V>::load(dy + at[u]);
             }
+            if (last) IO<T, V>::template put<NT>(last, kept);
             float sum[V];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -555,14 +642,19 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
                 add(vx[u], d);
                 __builtin_amdgcn_sched_barrier(0);   // (one vector at a time is enough arithmetic: fewer registers, more waves)
             }
-            if (a.dres) IO<T, V>::store(dres + (size_t)i * a.C, sum);
+            if (a.dres) {
+                kept = IO<T, V>::pack(sum);
+                last = dres + (size_t)i * a.C;
+            }
         }
+        if (last) IO<T, V>::template put<NT>(last, kept);
     } else if (pc.on) {
         constexpr int R = 4;
         const size_t step = (size_t)a.PL * a.C;
-        const int mine = max(0, ((int)pc.ni - pc.pl + a.PL - 1) / a.PL);
+        const int mine = vectors_of(a, pc);
         size_t o = (size_t)(pc.i0 + pc.pl) * a.C;
         int i = 0;
+#pragma unroll 1
         for (; i + R <= mine; i += R, o += R * step) {
             typename IO<T, V>::raw vx[R], vd[R];
 #pragma unroll
@@ -585,10 +677,16 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
         }
     }
     float *cp = a.cpart ? a.cpart + ((size_t)pc.n * a.gnblk + pc.blk) * 2 * a.C : nullptr;
-    join_grads<kT, V, A>(a, pc, t1, t2, rs, sh1, sh2, s1, s2, cp, cp ? cp + a.C : nullptr);
+    join_grads<V, A>(a, pc, t1, t2, rs, sh1, sh2, s1, s2, cp, cp ? cp + a.C : nullptr);
     __syncthreads();
     float2 *out = a.gpart + ((size_t)pc.n * a.gnblk + pc.blk) * a.G + pc.g0(a);
     for (int g = threadIdx.x; g < pc.ng; g += kT) out[g] = make_float2(s1[g], s2[g]);
+}
+
+template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds__(kT) void k_gn_bwd_reduce(const Args a)
+{
+    __shared__ float sh1[kT * (V + 1)], sh2[kT * (V + 1)], s1[kT * A], s2[kT * A];
+    grads_of_range<T, V, A, ACT, NT>(a, blockIdx.x, sh1, sh2, s1, s2);
 }
 
 __device__ __forceinline__ float2 join_group_grads(const Args &a, int n, int g, int k, int tpg)
@@ -596,6 +694,7 @@ __device__ __forceinline__ float2 join_group_grads(const Args &a, int n, int g, 
     const float2 *p = a.gpart + (size_t)n * a.gnblk * a.G + g;
     const float m = (float)((double)a.hw * a.D);
     float u1 = 0.0f, u2 = 0.0f;
+#pragma unroll 4
     for (int i = k; i < a.gnblk; i += tpg) {
         const float2 v = p[(size_t)i * a.G];
         u1 += v.x;
@@ -614,7 +713,7 @@ static __global__ __launch_bounds__(kT) void k_gn_bwd_finish(const Args a)
 }
 
 // dx of one vector
-template <typename T, int V, int A, int ACT>
+template <typename T, int V, int A, int ACT, bool NT>
 __device__ __forceinline__ void dx_store(const Args &a, const float (&f)[V], const float (&d)[V], const float (&mu)[A], const float (&rs)[A],
                                          const float (&k)[V], const float (&b)[V], const float (&u1)[A], const float (&u2)[A], T *dx)
 {
@@ -624,16 +723,27 @@ __device__ __forceinline__ void dx_store(const Args &a, const float (&f)[V], con
     // rstd (w dz - u1 - xc rstd u2) with k = rstd w, u1 and u2 already times rstd and rstd^2
 #pragma unroll
     for (int j = 0; j < V; ++j) xc[j] = k[j] * dz[j] - (u1[j / S] + xc[j] * u2[j / S]);
-    IO<T, V>::store(dx, xc);
+    IO<T, V>::template store<NT>(dx, xc);
 }
 
 // ---- backward, second pass: dx
-template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) void k_gn_bwd_apply(const Args a)
+template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds__(kT) void k_gn_bwd_apply(const Args a)
 {
-    constexpr int S = V / A;
+    typedef typename IO<T, V>::raw raw;
     __shared__ float s1[kT * A], s2[kT * A];
     const Place pc(a, blockIdx.x, V);
-    const int g0 = pc.g0(a);
+    const int mine = vectors_of(a, pc), g0 = pc.g0(a);
+    const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0 + (size_t)(pc.i0 + pc.pl) * a.C, step = (size_t)a.PL * a.C;
+    const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base;
+    T *dx = (T *)a.y + base;
+    Ahead<2, raw, 2> w;
+    auto get = [&](raw (&v)[2][2], int u, int i) {
+        v[0][u] = IO<T, V>::template load<NT>(x + i * step);
+        v[1][u] = IO<T, V>::template load<NT>(dy + i * step);
+    };
+    w.start(mine, get);
+    float mu[A], rs[A], k[V], b[V], u1[A], u2[A];
+    saved<V, A>(a, pc, mu, rs, k, b);
     if (a.finished) {
         for (int g = threadIdx.x; g < pc.ng; g += kT) {
             const float2 v = a.gsum[(size_t)pc.n * a.G + g0 + g];
@@ -641,7 +751,7 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
             s2[g] = v.y;
         }
     } else {
-        by_group(kT, pc.ng, [&](int g, int k, int tpg) {
+        by_group(pc.ng, [&](int g, int k, int tpg) {
             const float2 v = join_group_grads(a, pc.n, g0 + g, k, tpg);
             if (k == 0) {
                 s1[g] = v.x;
@@ -649,47 +759,20 @@ template <typename T, int V, int A, int ACT> __global__ __launch_bounds__(kT) vo
             }
         });
     }
-    float mu[A], rs[A], k[V], b[V], u1[A], u2[A];
-    saved<V, A>(a, pc, mu, rs, k, b);
     __syncthreads();
     if (!pc.on) return;
-    const int sg = a.D / S;
 #pragma unroll
     for (int j = 0; j < A; ++j) {
-        const int g = (pc.lv * A + j) / sg;
+        const int g = (int)a.by_sg.of((unsigned)(pc.lv * A + j));
         u1[j] = s1[g] * rs[j];
         u2[j] = s2[g] * rs[j] * rs[j];
     }
-    const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0;
-    const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base;
-    T *dx = (T *)a.y + base;
-    constexpr int R = 4;
-    const size_t step = (size_t)a.PL * a.C;
-    const int mine = max(0, ((int)pc.ni - pc.pl + a.PL - 1) / a.PL);
-    size_t o = (size_t)(pc.i0 + pc.pl) * a.C;
-    int i = 0;
-    for (; i + R <= mine; i += R, o += R * step) {
-        typename IO<T, V>::raw vx[R], vd[R];
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            vx[u] = IO<T, V>::load(x + o + u * step);
-            vd[u] = IO<T, V>::load(dy + o + u * step);
-        }
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            float f[V], d[V];
-            IO<T, V>::open(vx[u], f);
-            IO<T, V>::open(vd[u], d);
-            dx_store<T, V, A, ACT>(a, f, d, mu, rs, k, b, u1, u2, dx + o + u * step);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    for (; i < mine; ++i, o += step) {
+    w.run(mine, get, [&](raw (&v)[2][2], int u, int i) {
         float f[V], d[V];
-        IO<T, V>::open(IO<T, V>::load(x + o), f);
-        IO<T, V>::open(IO<T, V>::load(dy + o), d);
-        dx_store<T, V, A, ACT>(a, f, d, mu, rs, k, b, u1, u2, dx + o);
-    }
+        IO<T, V>::open(v[0][u], f);
+        IO<T, V>::open(v[1][u], d);
+        dx_store<T, V, A, ACT, NT>(a, f, d, mu, rs, k, b, u1, u2, dx + i * step);
+    });
 }
 
 // ---- dw / db from cpart: row r of the result (r = sample, or the one row) adds `rows` partial rows
@@ -724,7 +807,7 @@ static __global__ __launch_bounds__(1024) void k_gn_affine_grad(const float *__r
     }
 }
 
-// ---- a slab of a sample in the registers of one workgroup: one pass.  R vectors a thread, NT threads
+// ---- a slab of a sample in the registers of one workgroup: one pass.  R vectors a thread
 // pixel of a thread's vector r: every PL-th pixel, or -- quad -- four of every PL-th 2 x 2 block
 template <int R> __device__ __forceinline__ bool held_at(const Args &a, const Place &pc, int r, unsigned &pix)
 {
@@ -735,15 +818,15 @@ template <int R> __device__ __forceinline__ bool held_at(const Args &a, const Pl
     }
     const unsigned i = (unsigned)(pc.pl + (r >> 2) * a.PL);
     const bool ok = pc.on && i < (unsigned)a.items;
-    const unsigned h = row_of(a, i);
+    const unsigned h = a.by_w2.of(i);
     pix = 2 * (i + h * (unsigned)a.W2) + (r & 1) + ((r & 2) ? 2 * (unsigned)a.W2 : 0u);
     return ok;
 }
 
-template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_bounds__(NT) void k_gn_one(const Args a)
+template <typename T, int V, int A, int ACT, int R> __global__ __launch_bounds__(kT) void k_gn_one(const Args a)
 {
     constexpr int S = V / A;
-    __shared__ float sh[NT * (A + 1)], s_mean[NT * A], s_m2[NT * A];
+    __shared__ float sh[kT * (A + 1)], s_mean[kT * A], s_m2[kT * A];
     const Place pc(a, blockIdx.x, V);
     const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0;
     const T *x = (const T *)a.x + base;
@@ -788,11 +871,11 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
     for (int r = 0; r < R; ++r) keep(v[r]);
     float k[V], b[V], mu[A];
     affine<V>(a, pc, k, b);
-    join_threads<NT, V, A>(a, pc, st, (float)mine, (float)a.hw, sh, s_mean, s_m2);
+    join_threads<V, A>(a, pc, st, (float)mine, (float)a.hw, sh, s_mean, s_m2);
     __syncthreads();
     const int g0 = pc.g0(a);
     const float m = (float)((double)a.hw * a.D);
-    for (int g = threadIdx.x; g < pc.ng; g += NT) {
+    for (int g = threadIdx.x; g < pc.ng; g += kT) {
         const float rs = 1.0f / sqrtf(s_m2[g] / m + a.eps);
         a.mean[(size_t)pc.n * a.G + g0 + g] = s_mean[g];
         a.rstd[(size_t)pc.n * a.G + g0 + g] = rs;
@@ -800,10 +883,9 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
     }
     __syncthreads();
     if (!pc.on) return;
-    const int sg = a.D / S;
 #pragma unroll
     for (int j = 0; j < A; ++j) {
-        const int g = (pc.lv * A + j) / sg;
+        const int g = (int)a.by_sg.of((unsigned)(pc.lv * A + j));
         mu[j] = s_mean[g];
 #pragma unroll
         for (int u = 0; u < S; ++u) k[j * S + u] *= s_m2[g];
@@ -817,17 +899,17 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
             float f[V];
             IO<T, V>::open(v[r], f);
             const unsigned i = a.quad ? (unsigned)(pc.pl + (r >> 2) * a.PL) : p;
-            finish_store<T, V, A, ACT>(a, f, mu, k, b, res ? res + (size_t)i * a.C : nullptr, y + (size_t)p * a.C);
-            __builtin_amdgcn_sched_barrier(0);
+            typename IO<T, V>::raw q = {};
+            if (res) q = IO<T, V>::load(res + (size_t)i * a.C);
+            finish_store<T, V, A, ACT, false>(a, f, mu, k, b, res != nullptr, q, y + (size_t)p * a.C);
         }
     }
 }
 
 // the backward in one pass: x and dy of the slab in registers; with an affine of its own a sample writes dw / db, else cpart rows
-template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_bounds__(NT) void k_gn_bwd_one(const Args a)
+template <typename T, int V, int A, int ACT, int R> __global__ __launch_bounds__(kT) void k_gn_bwd_one(const Args a)
 {
-    constexpr int S = V / A;
-    __shared__ float sh1[NT * (V + 1)], sh2[NT * (V + 1)], s1[NT * A], s2[NT * A];
+    __shared__ float sh1[kT * (V + 1)], sh2[kT * (V + 1)], s1[kT * A], s2[kT * A];
     const Place pc(a, blockIdx.x, V);
     const size_t base = (size_t)pc.n * a.hw * a.C + pc.c0;
     const T *x = (const T *)a.x + base, *dy = (const T *)a.dy + base;
@@ -871,15 +953,14 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
         o1 = a.cpart + (size_t)pc.n * 2 * a.C;
         o2 = o1 + a.C;
     }
-    join_grads<NT, V, A>(a, pc, t1, t2, rs, sh1, sh2, s1, s2, o1, o2);
+    join_grads<V, A>(a, pc, t1, t2, rs, sh1, sh2, s1, s2, o1, o2);
     __syncthreads();
     if (!pc.on) return;
-    const int sg = a.D / S;
     const float m = (float)((double)a.hw * a.D);
     float u1[A], u2[A];
 #pragma unroll
     for (int j = 0; j < A; ++j) {
-        const int g = (pc.lv * A + j) / sg;
+        const int g = (int)a.by_sg.of((unsigned)(pc.lv * A + j));
         u1[j] = s1[g] / m * rs[j];
         u2[j] = s2[g] / m * rs[j] * rs[j];
     }
@@ -892,7 +973,7 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
             float f[V], d[V];
             IO<T, V>::open(vx[r], f);
             IO<T, V>::open(vd[r], d);
-            dx_store<T, V, A, ACT>(a, f, d, mu, rs, k, b, u1, u2, dx + (size_t)p * a.C);
+            dx_store<T, V, A, ACT, false>(a, f, d, mu, rs, k, b, u1, u2, dx + (size_t)p * a.C);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -910,16 +991,16 @@ template <typename T, int V, int A, int ACT, int R, int NT> __global__ __launch_
                 IO<T, V>::open(vd[r + 3], d3);
 #pragma unroll
                 for (int j = 0; j < V; ++j) d0[j] = ((d0[j] + d1[j]) + d2[j]) + d3[j];
-                IO<T, V>::store(dres + (size_t)(pc.pl + (r >> 2) * a.PL) * a.C, d0);
+                IO<T, V>::template store<false>(dres + (size_t)(pc.pl + (r >> 2) * a.PL) * a.C, d0);
             }
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ launches (one per element type)
-// what the host chose: vector, segments, and for the one-pass kernels how a slab is held (nt = 0: two passes)
+// what the host chose: vector, segments, and the vectors a thread of the one-pass kernels holds
 struct Choice {
-    int V, A, nt, R;
+    int V, A, R;
 };
 struct Runner {
     void (*stats)(const Args &, int V, int A, hipStream_t);

@@ -33,22 +33,42 @@ static void pick_vec(int C, int D, int dtype, uintptr_t bits, int &V, int &A)
 // channels that are whole groups and whole vectors
 static long long unit_of(int D, int V) { return (long long)D / gcd_ll(V, D) * V; }
 
-static void set_slab(Args &a, long long SC, int V, int nt)
+static void set_slab(Args &a, long long SC, int V)
 {
     a.SC = (int)SC;
     a.nslab = (int)((a.C + SC - 1) / SC);
     a.LV = (int)(SC / V);
-    a.PL = nt / a.LV;
+    a.PL = kT / a.LV;
+    a.by_lv.set((unsigned)a.LV);
+    a.by_pl.set((unsigned)a.PL);
+    a.by_nslab.set((unsigned)a.nslab);
+}
+
+static void set_ranges(Args &a, int nblk, long long per)
+{
+    a.nblk = nblk;
+    a.per = per;
+    a.by_nblk.set((unsigned)nblk);
 }
 
 // two passes: all channels if a workgroup's vectors reach over them, else as many whole groups as they do.  false: a group is wider
 static bool wide_slab(Args &a, int V)
 {
     const long long unit = unit_of(a.D, V), most = (long long)kT * V;
-    if (a.C <= most) set_slab(a, a.C, V, kT);
-    else if (unit <= most) set_slab(a, most / unit * unit, V, kT);
+    if (a.C <= most) set_slab(a, a.C, V);
+    else if (unit <= most) set_slab(a, most / unit * unit, V);
     else return false;
     return true;
+}
+
+constexpr long long kMostRanges = 4096;   // of a sample
+constexpr long long kLeast = 16384;       // values of a range at least
+constexpr int kJoin = 32;                 // ranges a sample up to which the second pass joins them itself
+
+static void set_groups(Args &a, const Choice &c)
+{
+    a.by_d.set((unsigned)a.D);
+    a.by_sg.set((unsigned)(a.D / (c.V / c.A)));
 }
 
 static void set_items(Args &a, int res_w, bool quad)
@@ -56,59 +76,62 @@ static void set_items(Args &a, int res_w, bool quad)
     a.quad = quad;
     a.items = quad ? a.hw / 4 : a.hw;
     a.W2 = res_w / 2;
-    if (quad && a.W2 > 1) {
-        int l = 0;
-        while ((1LL << l) < a.W2) ++l;
-        a.magic = (unsigned)(((1ULL << (31 + l)) / (unsigned)a.W2) + 1);   // exact for i < 2^31
-        a.shift = (unsigned)(l - 1);
-    }
+    if (quad) a.by_w2.set((unsigned)a.W2);
 }
 
-// ranges of a sample: about `goal` values a workgroup, `pixels` an item
-static int ranges_of(long long items, long long pixels, int C, int nslab, long long goal, long long &per)
+// Ranges of a sample in a kernel: about total / `share` values a workgroup, within [least, most]
+static void take_ranges(Args &a, double share, long long least, long long most)
 {
-    long long nblk = (long long)(((double)items * (double)(pixels * C) / nslab + goal - 1) / goal);
-    nblk = std::max(1LL, std::min(nblk, std::min(std::max(items, 1LL), 4096LL / std::min(nslab, 64))));
-    per = std::max(1LL, (items + nblk - 1) / nblk);
-    return (int)std::max(1LL, (items + per - 1) / per);
+    const long long items = a.items;
+    const double sample = (double)a.hw * a.C, goal = std::min(std::max(sample * a.N / share, (double)least), (double)most);
+    long long nblk = (long long)(sample / a.nslab / goal + 0.999);
+    nblk = std::max(1LL, std::min(std::min(nblk, std::max(items, 1LL)), kMostRanges));
+    const long long per = std::max(1LL, (items + nblk - 1) / nblk);
+    set_ranges(a, (int)std::max(1LL, (items + per - 1) / per), per);
 }
-
-constexpr long long kGoal = 32768;   // values of a workgroup's range in the two-pass kernels
-constexpr int kJoin = 32;            // ranges a sample up to which the second pass joins them itself
 
 // rows of partial sums a sample that any choice below may need (the workspace is sized before the pointers are known)
-static long long most_rows(long long HW, int C, int)
+static long long most_rows(long long HW, int C)
 {
-    return std::max(1LL, std::min(std::max(HW, 1LL), std::min(4096LL, (long long)((double)HW * C / kGoal) + 2)));
+    return std::max(1LL, std::min(std::max(HW, 1LL), std::min(kMostRanges, (long long)((double)HW * C / kLeast) + 2)));
 }
 
-// one pass: the narrowest slab of whole groups whose rows are `row` bytes, if a workgroup's registers hold it
-static bool hold(Args &a, int V, int esize, int row, Choice &c, const int (&R)[3])
+// One pass: slabs of whole groups whose rows are `row` bytes, if a workgroup holds one with R vectors a thread
+static bool hold(Args &a, int V, int esize, int row, int R, Choice &c)
 {
     const long long unit = unit_of(a.D, V);
     long long SC = unit;
     while (SC * esize < row && SC < a.C) SC += unit;
-    if (SC > a.C) SC = a.C;
-    static const int nts[3] = {256, 256, 1024};
-    for (int k = 0; k < 3; ++k) {
-        if (SC > (long long)nts[k] * V) continue;
-        set_slab(a, SC, V, nts[k]);
-        const long long need = (a.items + a.PL - 1) / a.PL * (a.quad ? 4 : 1);
-        if (need <= R[k]) {
-            c.nt = nts[k];
-            c.R = R[k];
-            return true;
-        }
-    }
-    return false;
+    if (SC > (long long)kT * V) return false;
+    set_slab(a, SC, V);
+    c.R = R;
+    return (a.items + a.PL - 1) / a.PL * (a.quad ? 4 : 1) <= R;
 }
 
-static int check_shape(long long N, long long HW, int C, int G, int dtype)
+// Rows of 128 bytes are whole cache lines; rows of 64 give twice the workgroups, which is what a small call lacks.  Forward / forward and
+// backward of 16x16x1024 bf16 with a half-resolution residual: one sample 6.5 / 13.2 us with 64-byte rows of 4 vectors, 9.5 / 18.4 with
+// 128-byte rows of 8 (9.8 / 24.7 in two passes); 64 samples 24.3 / 75.6 and 18.9 / 48.7 (22.8 / 71.3).  8x4x512, 16 samples: 6.0 / 12.6,
+// two passes 9.4 / 23.0
+static bool one_pass(Args &a, const m355_gn_desc *d, int V, int esize, Choice &c)
 {
+    if (hold(a, V, esize, 128, 4, c)) return true;
+    if (hold(a, V, esize, 64, 4, c) && (long long)a.N * a.nslab <= 1024) return true;
+    return hold(a, V, esize, 128, 8, c) || hold(a, V, esize, 64, 8, c);
+}
+
+static int check_desc(const m355_gn_desc *d)
+{
+    M355_REQUIRE(d, "group_norm: null pointer");
+    const long long N = d->N, HW = d->HW;
+    const int C = d->C, G = d->G, dtype = d->dtype;
     M355_REQUIRE(N >= 0 && HW >= 0 && C > 0 && G > 0, "group_norm: N %lld, HW %lld, C %d, G %d", N, HW, C, G);
     M355_REQUIRE(C % G == 0, "group_norm: %d channels in %d groups", C, G);
     M355_REQUIRE(dtype == M355_F32 || dtype == M355_F16 || dtype == M355_BF16, "group_norm: unknown dtype %d", dtype);
     M355_REQUIRE(N < (1LL << 31) && HW < (1LL << 36) && C <= (1 << 20), "group_norm: N %lld, HW %lld or C %d too large", N, HW, C);
+    M355_REQUIRE(d->act == 0 || d->act == 1, "group_norm: unknown activation %d", d->act);
+    M355_REQUIRE(d->aff_stride >= 0, "group_norm: the affine's rows are %lld floats apart", d->aff_stride);
+    M355_REQUIRE(d->res_w >= 0 && (d->res_w == 0 || (d->res_w % 2 == 0 && HW % (2LL * d->res_w) == 0)),
+                 "group_norm: a half-resolution residual needs even height and width (width %d, %lld pixels)", d->res_w, HW);
     return M355_OK;
 }
 
@@ -142,6 +165,11 @@ template <typename F> static void by_samples(const Args &all, int esize, F f)
     }
 }
 
+// A call whose inputs (`bytes` a value) come near the memory-side cache's 256 MB gains nothing from leaving its outputs there: written past
+// it, they neither push out what the second pass reads again nor are written back under the next kernel.  64x256x128x64 bf16: the four
+// kernels 487 -> 436 us; at 32 samples (134 MB in and out) past the cache is as fast as through it, below that slower for who reads y next.
+static bool past_cache(const m355_gn_desc *d, int bytes) { return (double)d->N * (double)d->HW * d->C * bytes >= 160e6; }
+
 static unsigned wave_grid(const Args &a) { return (unsigned)(((long long)a.N * a.G + kT / 64 - 1) / (kT / 64)); }
 
 static void affine_grad(const Args &a, hipStream_t s)
@@ -161,33 +189,38 @@ static void affine_grad(const Args &a, hipStream_t s)
 
 using namespace m355;
 
-extern "C" size_t m355_group_norm_ws_bytes(long long N, long long HW, int C, int G, int dtype, int backward)
+extern "C" size_t m355_group_norm_ws_bytes(const m355_gn_desc *d, int backward)
 {
-    if (gn::check_shape(N, HW, C, G, dtype) != M355_OK) return 0;
-    const size_t rows = (size_t)N * (size_t)gn::most_rows(HW, C, G);
-    size_t bytes = rows * (size_t)G * sizeof(float2);
-    if (backward) bytes += rows * 2 * (size_t)C * sizeof(float) + (size_t)N * G * sizeof(float2);
-    return bytes > 0 ? bytes : 8;
+    if (gn::check_desc(d) != M355_OK) return 0;
+    const size_t N = (size_t)d->N, rows = N * (size_t)gn::most_rows(d->HW, d->C);
+    size_t bytes = (rows + N) * (size_t)d->G * sizeof(float2);
+    if (backward) bytes += rows * 2 * (size_t)d->C * sizeof(float);
+    return (bytes + 15) / 16 * 16;
 }
 
-extern "C" int m355_group_norm_fwd(const void *x, const float *w, const float *b, long long aff_stride, float w_off, const void *res,
-                                   int res_w, void *y, float *mean, float *rstd, void *ws, long long N, long long HW, int C, int G,
-                                   float eps, int act, float slope, float out_slope, int dtype, void *stream)
+static void fill(gn::Args &a, const m355_gn_desc *d, const void *x, const float *w, const float *b, float *stat)
 {
-    const int rc = gn::check_shape(N, HW, C, G, dtype);
+    a.x = x; a.w = w; a.b = b; a.mean = stat; a.rstd = stat + (size_t)d->N * d->G;
+    a.aff_stride = d->aff_stride; a.hw = d->HW; a.N = (int)d->N; a.C = d->C; a.G = d->G; a.D = d->C / d->G; a.act = d->act;
+    a.w_off = d->w_off; a.eps = d->eps; a.slope = d->slope; a.out_slope = d->out_slope; a.per_sample = d->per_sample != 0;
+}
+
+extern "C" int m355_group_norm_fwd(const m355_gn_desc *d, const void *x, const float *w, const float *b, const void *res, void *y, float *stat,
+                                   void *ws, void *stream)
+{
+    const int rc = gn::check_desc(d);
     if (rc != M355_OK) return rc;
-    if (N == 0 || HW == 0) return M355_OK;
-    M355_REQUIRE(x && y && mean && rstd && ws, "group_norm_fwd: null pointer");
+    if (d->N == 0 || d->HW == 0) return M355_OK;
+    M355_REQUIRE(x && y && stat && ws, "group_norm_fwd: null pointer");
     M355_REQUIRE(x != y, "group_norm_fwd: y must not be x");
-    M355_REQUIRE(act == 0 || act == 1, "group_norm_fwd: unknown activation %d", act);
-    M355_REQUIRE(res_w >= 0 && (res_w == 0 || (res && res_w % 2 == 0 && HW % (2LL * res_w) == 0)),
-                 "group_norm_fwd: a half-resolution residual needs even height and width (width %d, %lld pixels)", res_w, HW);
+    M355_REQUIRE(d->res_w == 0 || res, "group_norm_fwd: res_w without a residual");
     gn::Args a = {};
-    a.x = x; a.res = res; a.y = y; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd; a.gpart = (float2 *)ws;
-    a.aff_stride = aff_stride; a.hw = HW; a.N = (int)N; a.C = C; a.G = G; a.D = C / G; a.act = act;
-    a.w_off = w_off; a.eps = eps; a.slope = slope; a.out_slope = out_slope;
+    fill(a, d, x, w, b, stat);
+    a.res = res; a.y = y; a.gpart = (float2 *)ws;
+    const int C = d->C, dtype = d->dtype, res_w = d->res_w;
     gn::Choice c = {};
     gn::pick_vec(C, a.D, dtype, (uintptr_t)x | (uintptr_t)y | (uintptr_t)res, c.V, c.A);
+    gn::set_groups(a, c);
     if (!gn::wide_slab(a, c.V)) {
         set_error("group_norm_fwd: groups of %d channels (vectors of %d) are wider than a workgroup takes", a.D, c.V);
         return M355_ERR_UNSUPPORTED;
@@ -195,11 +228,10 @@ extern "C" int m355_group_norm_fwd(const void *x, const float *w, const float *b
     const gn::Runner run = gn::runner(dtype);
     hipStream_t s = (hipStream_t)stream;
     const int es = gn::elem_bytes(dtype);
-    static const int R[3] = {4, 16, 16};
     gn::set_items(a, res_w, res_w > 0);
-    a.nblk = a.gnblk = 1;
-    a.per = a.items;
-    if (gn::hold(a, c.V, es, 128, c, R) || gn::hold(a, c.V, es, 64, c, R)) {
+    gn::set_ranges(a, 1, a.items);
+    a.gnblk = 1;
+    if (gn::one_pass(a, d, c.V, es, c)) {
         gn::by_samples(a, es, [&](const gn::Args &p) { run.one(p, c, s); });
         return check_launch("group_norm_fwd");
     }
@@ -207,10 +239,11 @@ extern "C" int m355_group_norm_fwd(const void *x, const float *w, const float *b
     gn::Args st = a;
     gn::set_items(st, 0, false);
     st.res = nullptr;
-    st.nblk = gn::ranges_of(st.items, 1, C, st.nslab, gn::kGoal, st.per);
+    gn::take_ranges(st, 512, 16384, 131072);
     st.gnblk = a.gnblk = st.nblk;
     st.gper = a.gper = st.per;
-    a.nblk = gn::ranges_of(a.items, a.quad ? 4 : 1, C, a.nslab, gn::kGoal, a.per);
+    gn::take_ranges(a, 1024, 16384, 32768);
+    a.nt = gn::past_cache(d, es);
     a.finished = a.gnblk > gn::kJoin;
     gn::by_samples(st, es, [&](const gn::Args &p) { run.stats(p, c.V, c.A, s); });
     if (a.finished)
@@ -219,26 +252,23 @@ extern "C" int m355_group_norm_fwd(const void *x, const float *w, const float *b
     return check_launch("group_norm_fwd");
 }
 
-extern "C" int m355_group_norm_bwd(const void *dy, const void *x, const float *w, const float *b, long long aff_stride, float w_off,
-                                   const float *mean, const float *rstd, void *dx, float *dw, float *db, int per_sample, void *dres,
-                                   int res_w, void *ws, long long N, long long HW, int C, int G, int act, float slope, int dtype,
-                                   void *stream)
+extern "C" int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const void *x, const float *w, const float *b, const float *stat,
+                                   void *dx, float *dw, float *db, void *dres, void *ws, void *stream)
 {
-    const int rc = gn::check_shape(N, HW, C, G, dtype);
+    const int rc = gn::check_desc(d);
     if (rc != M355_OK) return rc;
-    if (N == 0 || HW == 0) return M355_OK;   // (the caller zeroes dw / db of an empty batch)
-    M355_REQUIRE(dy && x && mean && rstd && ws, "group_norm_bwd: null pointer");
+    if (d->N == 0 || d->HW == 0) return M355_OK;   // (the caller zeroes dw / db of an empty batch)
+    M355_REQUIRE(dy && x && stat && ws, "group_norm_bwd: null pointer");
     M355_REQUIRE(dx != x && dx != dy, "group_norm_bwd: dx must be a tensor of its own");
-    M355_REQUIRE(act == 0 || act == 1, "group_norm_bwd: unknown activation %d", act);
-    M355_REQUIRE(res_w >= 0 && (res_w == 0 ? !dres : res_w % 2 == 0 && HW % (2LL * res_w) == 0),
-                 "group_norm_bwd: a half-resolution residual needs even height and width (width %d, %lld pixels)", res_w, HW);
+    M355_REQUIRE(!dres || d->res_w > 0, "group_norm_bwd: dres is the gradient of a half-resolution residual");
     gn::Args a = {};
-    a.x = x; a.dy = dy; a.y = dx; a.dres = dres; a.w = w; a.b = b; a.mean = (float *)mean; a.rstd = (float *)rstd;
-    a.aff_stride = aff_stride; a.hw = HW; a.N = (int)N; a.C = C; a.G = G; a.D = C / G; a.act = act;
-    a.w_off = w_off; a.slope = slope; a.out_slope = 1.0f;
-    a.dw = dw; a.db = db; a.per_sample = per_sample != 0;
+    fill(a, d, x, w, b, (float *)stat);
+    a.dy = dy; a.y = dx; a.dres = dres; a.dw = dw; a.db = db;
+    const long long N = d->N, HW = d->HW;
+    const int C = d->C, G = d->G, dtype = d->dtype, res_w = d->res_w;
     gn::Choice c = {};
     gn::pick_vec(C, a.D, dtype, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dres, c.V, c.A);
+    gn::set_groups(a, c);
     if (!gn::wide_slab(a, c.V)) {
         set_error("group_norm_bwd: groups of %d channels (vectors of %d) are wider than a workgroup takes", a.D, c.V);
         return M355_ERR_UNSUPPORTED;
@@ -247,32 +277,32 @@ extern "C" int m355_group_norm_bwd(const void *dy, const void *x, const float *w
     hipStream_t s = (hipStream_t)stream;
     const int es = gn::elem_bytes(dtype);
     a.gpart = (float2 *)ws;
-    a.gsum = a.gpart + (size_t)N * gn::most_rows(HW, C, G) * G;
+    a.gsum = a.gpart + (size_t)N * gn::most_rows(HW, C) * G;
     float *cpart = (float *)(a.gsum + (size_t)N * G);
     a.cpart = dw || db ? cpart : nullptr;
-    static const int R[3] = {4, 8, 8};
     gn::set_items(a, res_w, res_w > 0);   // (the same order of additions whether or not dres is wanted)
-    a.nblk = a.gnblk = 1;
-    a.per = a.items;
-    if (gn::hold(a, c.V, es, 128, c, R) || gn::hold(a, c.V, es, 64, c, R)) {
+    gn::set_ranges(a, 1, a.items);
+    a.gnblk = 1;
+    if (gn::one_pass(a, d, c.V, es, c)) {
         gn::by_samples(a, es, [&](const gn::Args &p) { run.bwd_one(p, c, s); });
         if (!a.per_sample && a.cpart) gn::affine_grad(a, s);
         return check_launch("group_norm_bwd");
     }
     gn::wide_slab(a, c.V);
-    a.nblk = gn::ranges_of(a.items, a.quad ? 4 : 1, C, a.nslab, gn::kGoal, a.per);
+    gn::take_ranges(a, 512, 16384, 32768);
     a.gnblk = a.nblk;
-    a.finished = a.gnblk > gn::kJoin;
+    gn::Args p2 = a;
+    gn::set_items(p2, 0, false);
+    p2.dres = nullptr;
+    gn::take_ranges(p2, 1024, 16384, 32768);
+    a.nt = p2.nt = gn::past_cache(d, 2 * es);
+    a.finished = p2.finished = a.gnblk > gn::kJoin;
     gn::by_samples(a, es, [&](const gn::Args &p) { run.bwd_reduce(p, c.V, c.A, s); });
     if (a.cpart) gn::affine_grad(a, s);
     if (dx) {
         if (a.finished)
             gn::by_samples(a, es, [&](const gn::Args &p) { hipLaunchKernelGGL(gn::k_gn_bwd_finish, dim3(gn::wave_grid(p)), dim3(gn::kT), 0, s, p); });
-        gn::Args d = a;
-        gn::set_items(d, 0, false);
-        d.dres = nullptr;
-        d.nblk = gn::ranges_of(d.items, 1, C, d.nslab, gn::kGoal, d.per);
-        gn::by_samples(d, es, [&](const gn::Args &p) { run.bwd_apply(p, c.V, c.A, s); });
+        gn::by_samples(p2, es, [&](const gn::Args &p) { run.bwd_apply(p, c.V, c.A, s); });
     }
     return check_launch("group_norm_bwd");
 }

@@ -39,30 +39,37 @@ void stats(const Args &a, int V, int A, hipStream_t s)
 }
 void apply(const Args &a, int V, int A, hipStream_t s)
 {
-    by_all(V, A, a.act, [&](auto v, auto g, auto t) { hipLaunchKernelGGL((k_gn_apply<T, v(), g(), t()>), grid(a), dim3(kT), 0, s, a); });
+    by_all(V, A, a.act, [&](auto v, auto g, auto t) {
+        if (a.nt) hipLaunchKernelGGL((k_gn_apply<T, v(), g(), t(), true>), grid(a), dim3(kT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_apply<T, v(), g(), t(), false>), grid(a), dim3(kT), 0, s, a);
+    });
 }
 void bwd_reduce(const Args &a, int V, int A, hipStream_t s)
 {
-    by_all(V, A, a.act, [&](auto v, auto g, auto t) { hipLaunchKernelGGL((k_gn_bwd_reduce<T, v(), g(), t()>), grid(a), dim3(kT), 0, s, a); });
+    by_all(V, A, a.act, [&](auto v, auto g, auto t) {
+        if (a.nt) hipLaunchKernelGGL((k_gn_bwd_reduce<T, v(), g(), t(), true>), grid(a), dim3(kT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_bwd_reduce<T, v(), g(), t(), false>), grid(a), dim3(kT), 0, s, a);
+    });
 }
 void bwd_apply(const Args &a, int V, int A, hipStream_t s)
 {
-    by_all(V, A, a.act, [&](auto v, auto g, auto t) { hipLaunchKernelGGL((k_gn_bwd_apply<T, v(), g(), t()>), grid(a), dim3(kT), 0, s, a); });
+    by_all(V, A, a.act, [&](auto v, auto g, auto t) {
+        if (a.nt) hipLaunchKernelGGL((k_gn_bwd_apply<T, v(), g(), t(), true>), grid(a), dim3(kT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_bwd_apply<T, v(), g(), t(), false>), grid(a), dim3(kT), 0, s, a);
+    });
 }
 void one(const Args &a, const Choice &c, hipStream_t s)
 {
     by_all(c.V, c.A, a.act, [&](auto v, auto g, auto t) {
-        if (c.nt == 1024) hipLaunchKernelGGL((k_gn_one<T, v(), g(), t(), 16, 1024>), grid(a), dim3(1024), 0, s, a);
-        else if (c.R == 16) hipLaunchKernelGGL((k_gn_one<T, v(), g(), t(), 16, 256>), grid(a), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_gn_one<T, v(), g(), t(), 4, 256>), grid(a), dim3(256), 0, s, a);
+        if (c.R == 8) hipLaunchKernelGGL((k_gn_one<T, v(), g(), t(), 8>), grid(a), dim3(kT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_one<T, v(), g(), t(), 4>), grid(a), dim3(kT), 0, s, a);
     });
 }
 void bwd_one(const Args &a, const Choice &c, hipStream_t s)
 {
     by_all(c.V, c.A, a.act, [&](auto v, auto g, auto t) {
-        if (c.nt == 1024) hipLaunchKernelGGL((k_gn_bwd_one<T, v(), g(), t(), 8, 1024>), grid(a), dim3(1024), 0, s, a);
-        else if (c.R == 8) hipLaunchKernelGGL((k_gn_bwd_one<T, v(), g(), t(), 8, 256>), grid(a), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_gn_bwd_one<T, v(), g(), t(), 4, 256>), grid(a), dim3(256), 0, s, a);
+        if (c.R == 8) hipLaunchKernelGGL((k_gn_bwd_one<T, v(), g(), t(), 8>), grid(a), dim3(kT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_bwd_one<T, v(), g(), t(), 4>), grid(a), dim3(kT), 0, s, a);
     });
 }
 

@@ -5,19 +5,19 @@ any length up to 112 tensors, no host synchronisation, capturable.  No CPU or to
 
 `clip_grad_norm_` takes parameters as torch.nn.utils.clip_grad_norm_ does, `clip_grads_` the gradient tensors themselves (in place, or
 into `out` buffers with a scale: averaging a summed message and clipping it is one pass), `grad_norm` only measures."""
-import ctypes
+from array import array
 
 import torch
 
 from . import _lib
-from ._lib import launch, lib, ptr, stream
-from .group_norm import _DTYPES, _on
+from ._lib import launch, lib, stream
+from .group_norm import _DTYPES, on_device
+
+_strided = torch.strided
 
 
 def _flat(t):
     """the tensor's values lie in its memory without gaps, in whatever order (a permuted view counts)"""
-    if t.is_contiguous():
-        return True
     want = 1
     for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
         if st != want:
@@ -27,42 +27,50 @@ def _flat(t):
 
 
 def _check(tensors, what):
+    """-> the list, its device's index, and whether every tensor's values lie together"""
     ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    dev = None
+    index, together = None, True
     for t in ts:
-        if not torch.is_tensor(t) or not t.is_cuda:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise _lib.M355Error(f"{what}: gradients must be CUDA(HIP) tensors; there is no CPU implementation")
-        if t.layout != torch.strided:
+        if t.layout is not _strided:
             raise TypeError(f"{what}: a gradient is {t.layout}: dense tensors only")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{what}: gradients must be float32, float16 or bfloat16, got {t.dtype}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: gradients on {dev} and on {t.device}: clip each device's own list")
-    return ts, dev
+        d = t.get_device()
+        if d != index:
+            if index is not None:
+                raise ValueError(f"{what}: gradients on cuda:{index} and on {t.device}: clip each device's own list")
+            index = d
+        if together and not t.is_contiguous():
+            together = _flat(t) or t.numel() == 0
+    if not ts:
+        raise ValueError(f"{what}: no gradients")
+    return ts, index, together
 
 
-def _run(ts, outs, dev, max_norm, scale):
+def _run(ts, outs, index, max_norm, scale):
     n = len(ts)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    with _on(norm):
+    with on_device(index):
+        dev = ts[0].device
         ws = torch.empty((lib().m355_grad_clip_ws_bytes(n),), dtype=torch.uint8, device=dev)
-        args = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
-                None if outs is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs]),
-                (ctypes.c_longlong * n)(*[t.numel() for t in ts]), (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in ts])]
-        launch("grad_clip", *args, n, float(scale), float(max_norm), ptr(norm), ptr(ws), stream())
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ptrs = array("Q", [t.data_ptr() for t in ts])
+        optr = None if outs is None else ptrs if outs is ts else array("Q", [t.data_ptr() for t in outs])
+        nums, kinds = array("q", [t.numel() for t in ts]), array("i", [_DTYPES[t.dtype] for t in ts])
+        launch("grad_clip", ptrs.buffer_info()[0], None if outs is None else optr.buffer_info()[0], nums.buffer_info()[0],
+               kinds.buffer_info()[0], n, scale, max_norm, norm.data_ptr(), ws.data_ptr(), stream())
     return norm
 
 
 def grad_norm(grads, scale=1.0):
     """The 2-norm of all values of `grads` (a tensor or an iterable of tensors, float32 / float16 / bfloat16 mixed, one device), times
     |scale|: a 0-dimensional float32 tensor on their device.  Squares are added in 64 bits in a fixed order."""
-    ts, dev = _check(grads, "grad_norm")
-    if not ts:
-        raise ValueError("grad_norm: no gradients")
-    with torch.no_grad():
-        return _run([t if _flat(t) else t.contiguous() for t in ts], None, dev, 0.0, scale)
+    ts, index, together = _check(grads, "grad_norm")
+    if not together:
+        with torch.no_grad():
+            ts = [t.contiguous() for t in ts]
+    return _run(ts, None, index, 0.0, float(scale))
 
 
 def clip_grads_(grads, max_norm, out=None, scale=1.0):
@@ -72,25 +80,23 @@ def clip_grads_(grads, max_norm, out=None, scale=1.0):
     In place, or -- out: as many tensors of the same shapes, types and strides -- written there, the gradients left as they were.
     max_norm >= 0, infinity never clips.  An infinite norm makes the finite gradients 0, a NaN makes all of them NaN (as
     torch.nn.utils.clip_grad_norm_): the returned norm says so.  Tensors that share memory (the same gradient twice) are refused."""
-    ts, dev = _check(grads, "clip_grads_")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads_: max_norm={max_norm!r}")
-    if not ts:
-        raise ValueError("clip_grads_: no gradients")
-    outs = ts if out is None else _check(out, "clip_grads_")[0]
-    if len(outs) != len(ts):
-        raise ValueError(f"clip_grads_: {len(ts)} gradients, {len(outs)} outputs")
-    for t, o in zip(ts, outs):
-        if not _flat(t):
-            raise ValueError(f"clip_grads_: a gradient of shape {list(t.shape)} and strides {list(t.stride())} has gaps or repeats")
-        if o is not t and (o.device != dev or o.dtype != t.dtype or o.shape != t.shape
-                           or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))):
-            raise ValueError("clip_grads_: an output must have its gradient's device, type, shape and strides")
-    with torch.no_grad():
-        norm = _run(ts, outs, dev, max_norm, scale)
-        for o in outs:
-            torch.autograd.graph.increment_version(o)
+    ts, index, together = _check(grads, "clip_grads_")
+    if not together:
+        raise ValueError("clip_grads_: a gradient's values have gaps or repeats between them (an expanded or sliced view)")
+    outs = ts
+    if out is not None:
+        outs, o_index, _ = _check(out, "clip_grads_")
+        if len(outs) != len(ts) or o_index != index:
+            raise ValueError(f"clip_grads_: {len(ts)} gradients on cuda:{index}, {len(outs)} outputs on cuda:{o_index}")
+        for t, o in zip(ts, outs):
+            if o.dtype is not t.dtype or o.shape != t.shape or (
+                    not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride()):
+                raise ValueError("clip_grads_: an output must have its gradient's type, shape and strides")
+    norm = _run(ts, outs, index, max_norm, float(scale))
+    torch.autograd.graph.increment_version(outs)
     return norm
 
 

@@ -6,24 +6,20 @@ m355_group_norm_*) -- the batch-independent counterpart of gan_ops' fused batch 
 `group_norm_act` is the function, `GroupNorm2d` the conditional form behind `norm_g='group'` (gan.ConditionalBatchNorm2d) and
 `GroupNormAct2d` the layer with its own affine (norm_d='group', ReconstructionNetwork(norm='group')).  No CPU or torch fallback: CPU
 tensors raise."""
+import ctypes
+
 import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import launch, lib, ptr, stream
+from ._lib import launch, lib, stream
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # m355_dtype
 ACTS = {"lrelu": 0, "silu": 1}
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-class _on:
-    """launches go to the current stream of the tensor's device, whichever device is current"""
-
-    def __new__(cls, t):
-        return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else _NULL
-
-
-class _Null:
+class _Here:
     def __enter__(self):
         return None
 
@@ -31,89 +27,27 @@ class _Null:
         return False
 
 
-_NULL = _Null()
+_HERE = _Here()
 
 
-def _ws(n, hw, c, groups, dt, backward, dev):
-    nbytes = lib().m355_group_norm_ws_bytes(n, hw, c, groups, dt, backward)
-    return torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+def on_device(index):
+    """launches go to the current stream of the tensors' device, whichever device is current"""
+    return _HERE if index == _get_device() else torch.cuda.device(index)
 
 
-def _sizes(x):
-    n, c = x.shape[0], x.shape[-1]
-    return n, (x.numel() // (n * c) if x.numel() else 0), c
+class _Plan:
+    """what a call's shapes, types, strides and constants decide: the checked descriptor and the workspace sizes"""
+    __slots__ = ("desc", "at", "index", "stat", "ws", "ws_bwd", "half", "res_shape", "floats", "cast", "empty", "dtype")
 
 
-def _affine(t):
-    """[C] or [N,C] fp32 with unit channel stride -> the tensor itself (a view of a batched GEMM's output is read in place)"""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+_PLANS = {}   # by shapes, types, strides, devices and constants -- never by what the tensors hold or where they lie
 
 
-def _forward(x, weight, bias, res, groups, eps, act, slope, w_off, out_slope):
-    n, hw, c = _sizes(x)
-    dt = _DTYPES[x.dtype]
-    y = torch.empty_like(x)
-    stat = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
-    if x.numel() == 0:
-        return y, stat, weight, bias
-    weight = None if weight is None else _affine(weight)
-    bias = None if bias is None else _affine(bias)
-    one = weight if weight is not None else bias
-    stride = 0
-    if one is not None and one.dim() == 2:
-        stride = one.stride(0)
-        if weight is not None and bias is not None and bias.stride(0) != stride:
-            weight, bias = weight.contiguous(), bias.contiguous()
-            stride = c
-    res_w = 0
-    if res is not None and res.shape != x.shape:
-        res_w = x.shape[2]
-    with _on(x):
-        launch("group_norm_fwd", ptr(x), ptr(weight), ptr(bias), stride, w_off, ptr(res), res_w, ptr(y), stat.data_ptr(),
-               stat.data_ptr() + 4 * n * groups, ptr(_ws(n, hw, c, groups, dt, 0, x.device)), n, hw, c, groups, eps, act, slope,
-               out_slope, dt, stream())
-    return y, stat, weight, bias
+def _reset():
+    _PLANS.clear()
 
 
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, res, groups, eps, act, slope, w_off, out_slope):
-        y, stat, w, b = _forward(x, weight, bias, res, groups, eps, act, slope, w_off, out_slope)
-        ctx.save_for_backward(x, w, b, stat)
-        ctx.cfg = (groups, act, slope, w_off, None if res is None else tuple(res.shape))
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stat = ctx.saved_tensors
-        groups, act, slope, w_off, res_shape = ctx.cfg
-        n, hw, c = _sizes(x)
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        if dy.dtype != x.dtype:
-            dy = dy.to(x.dtype)
-        dy = dy.contiguous()
-        dev = x.device
-        dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(weight.shape, dtype=torch.float32, device=dev) if need_w else None
-        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if need_b else None
-        half = res_shape is not None and res_shape != tuple(x.shape)
-        dres = None
-        if need_r:
-            dres = torch.empty(res_shape, dtype=x.dtype, device=dev) if half else dy
-        if x.numel() == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif need_x or need_w or need_b or (half and need_r):
-            one = weight if weight is not None else bias
-            per_sample = one is not None and one.dim() == 2
-            with _on(x):
-                launch("group_norm_bwd", ptr(dy), ptr(x), ptr(weight), ptr(bias), one.stride(0) if per_sample else 0, w_off,
-                       stat.data_ptr(), stat.data_ptr() + 4 * n * groups, ptr(dx), ptr(dw), ptr(db), int(per_sample),
-                       ptr(dres) if half else None, x.shape[2] if half else 0, ptr(_ws(n, hw, c, groups, _DTYPES[x.dtype], 1, dev)),
-                       n, hw, c, groups, act, slope, _DTYPES[x.dtype], stream())
-        return dx, dw, db, dres, None, None, None, None, None, None
+_lib._RESET_HOOKS.append(_reset)
 
 
 def _check_affine(t, name, n, c, x):
@@ -123,10 +57,9 @@ def _check_affine(t, name, n, c, x):
         raise ValueError(f"group_norm_act: {name} must be [{c}] or [{n}, {c}], got {list(t.shape)}")
     if t.dtype not in _DTYPES:
         raise TypeError(f"group_norm_act: {name} must be float32, float16 or bfloat16, got {t.dtype}")
-    return t if t.dtype == torch.float32 else t.float()
 
 
-def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
+def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
     if not torch.is_tensor(x) or not x.is_cuda:
         raise _lib.M355Error("group_norm_act: x must be a CUDA(HIP) tensor; there is no CPU implementation")
     if x.dtype not in _DTYPES:
@@ -140,24 +73,121 @@ def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
         raise ValueError(f"group_norm_act: eps={eps!r}")
     if act not in ACTS:
         raise ValueError(f"group_norm_act: act={act!r} (one of {sorted(ACTS)})")
-    if weight is not None:
-        weight = _check_affine(weight, "weight", n, c, x)
-    if bias is not None:
-        bias = _check_affine(bias, "bias", n, c, x)
+    p = _Plan()
+    p.cast = False
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_affine(t, name, n, c, x)
+            p.cast = p.cast or t.dtype != torch.float32
+    one = weight if weight is not None else bias
     if weight is not None and bias is not None and weight.shape != bias.shape:
         raise ValueError(f"group_norm_act: weight {list(weight.shape)} and bias {list(bias.shape)} must have one shape")
+    # rows of unit channel stride, as far apart in weight as in bias, are read in place (views of a batched GEMM's output)
+    per_sample = one is not None and one.dim() == 2
+    aff = [t for t in (weight, bias) if t is not None]
+    plain = all(t.stride(-1) == 1 or c == 1 for t in aff) and (not per_sample or len({t.stride(0) for t in aff}) == 1) and not p.cast
+    p.floats = aff and not plain
+    half = False
     if res is not None:
         if not torch.is_tensor(res) or res.device != x.device or res.dtype != x.dtype:
             raise TypeError(f"group_norm_act: res must be {x.dtype} on {x.device}")
-        if res.shape != x.shape and not (x.dim() == 4 and x.shape[1] % 2 == 0 and x.shape[2] % 2 == 0
-                                         and tuple(res.shape) == (n, x.shape[1] // 2, x.shape[2] // 2, c)):
+        half = res.shape != x.shape
+        if half and not (x.dim() == 4 and x.shape[1] % 2 == 0 and x.shape[2] % 2 == 0
+                         and tuple(res.shape) == (n, x.shape[1] // 2, x.shape[2] // 2, c)):
             raise ValueError(f"group_norm_act: res must have x's shape {list(x.shape)} or half its height and width, got {list(res.shape)}")
+    p.empty = x.numel() == 0
+    p.half, p.res_shape = half, None if res is None else tuple(res.shape)
+    p.index, p.dtype = x.device.index, x.dtype
+    p.stat = 2 * n * groups
+    p.desc = _lib.GnDesc(n, 0 if p.empty else x.numel() // (n * c), (one.stride(0) if plain else c) if per_sample else 0, c, groups,
+                         _DTYPES[x.dtype], ACTS[act], x.shape[2] if half else 0, int(per_sample), float(eps), float(slope),
+                         float(out_slope), float(w_off))
+    p.at = ctypes.addressof(p.desc)
+    p.ws, p.ws_bwd = (0, 0) if p.empty else (lib().m355_group_norm_ws_bytes(p.at, 0), lib().m355_group_norm_ws_bytes(p.at, 1))
+    if not p.empty and not p.ws_bwd:
+        raise _lib.M355Error("group_norm_act: " + lib().m355_last_error().decode("utf-8", "replace"))
+    return p
+
+
+def _key(t):
+    return None if t is None else (t.shape, t.dtype, t.device, t.stride())
+
+
+def _forward(x, weight, bias, res, p):
+    y = torch.empty_like(x)
+    # (a small workspace lies behind the statistics: one allocation; a large one must not live as long as they do)
+    small = p.ws <= 65536
+    stat = torch.empty((p.stat + (-p.stat) % 4 + p.ws // 4 if small else p.stat,), dtype=torch.float32, device=x.device)
+    if not p.empty:
+        at = stat.data_ptr()
+        ws = None if small else torch.empty((p.ws,), dtype=torch.uint8, device=x.device)
+        with on_device(p.index):
+            launch("group_norm_fwd", p.at, x.data_ptr(), None if weight is None else weight.data_ptr(),
+                   None if bias is None else bias.data_ptr(), None if res is None else res.data_ptr(), y.data_ptr(), at,
+                   at + 4 * (p.stat + (-p.stat) % 4) if small else ws.data_ptr(), stream())
+    return y, stat
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, res, p):
+        y, stat = _forward(x, weight, bias, res, p)
+        ctx.save_for_backward(x, weight, bias, stat)
+        ctx.p = p
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stat = ctx.saved_tensors
+        p, dev = ctx.p, x.device
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        if dy.dtype != p.dtype:
+            dy = dy.to(p.dtype)
+        dy = dy.contiguous()
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty(weight.shape, dtype=torch.float32, device=dev) if need_w else None
+        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if need_b else None
+        dres = dy if need_r else None
+        if need_r and p.half:
+            dres = torch.empty(p.res_shape, dtype=p.dtype, device=dev)
+        if p.empty:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        elif need_x or need_w or need_b or (need_r and p.half):
+            ws = torch.empty((p.ws_bwd,), dtype=torch.uint8, device=dev)
+            with on_device(p.index):
+                launch("group_norm_bwd", p.at, dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
+                       None if bias is None else bias.data_ptr(), stat.data_ptr(), None if dx is None else dx.data_ptr(),
+                       None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+                       dres.data_ptr() if need_r and p.half else None, ws.data_ptr(), stream())
+        return dx, dw, db, dres, None
+
+
+def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
+    try:
+        key = (x.shape, x.dtype, x.device, int(num_groups), float(eps), act, float(slope), w_off, out_slope, _key(weight), _key(bias),
+               None if res is None else (res.shape, res.dtype, res.device))
+        p = _PLANS.get(key)
+    except (AttributeError, TypeError, ValueError):   # (not tensors, not numbers: the checks say what)
+        key = p = None
+    if p is None:
+        p = _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope)
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        if key is not None:
+            _PLANS[key] = p
+    if p.floats:
+        weight, bias = (None if t is None else t.float().contiguous() for t in (weight, bias))
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if res is not None and not res.is_contiguous():
         res = res.contiguous()
-    x = x.contiguous()
-    args = (x, weight, bias, res, groups, float(eps), ACTS[act], float(slope), float(w_off), float(out_slope))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
-        return _GroupNormAct.apply(*args)
-    return _forward(*args)[0]
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad) or (res is not None and res.requires_grad)):
+        return _GroupNormAct.apply(x, weight, bias, res, p)
+    return _forward(x, weight, bias, res, p)[0]
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu", slope=1.0, res=None):

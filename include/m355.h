@@ -561,23 +561,26 @@ int m355_ipc_allreduce(float *inout, int n, void *const *regions /*[world], host
                        int channel, unsigned *status /*device word*/, int timeout_ms, void *stream);
 
 /* ---- Group norm with an activation, channels last (the framework's own: the reference's norms are batch and instance norm,
- *      models/gan.py:268-277, 29-31).  x, y [N][HW][C] of `dtype` (m355_dtype, in both builds of the library); G groups of C / G
- *      neighbouring channels; statistics over the HW * C / G values of a (sample, group), 32-bit, without cancellation, in a fixed order.
+ *      models/gan.py:268-277, 29-31).  x, y [N][HW][C] of d->dtype (m355_dtype, in both builds of the library); G groups of C / G
+ *      neighbouring channels; statistics over the HW * C / G values of a (sample, group), 32-bit, without cancellation, in a fixed order:
  *          y = act((x - mean) rstd * (w_off + w) + b) [+ res], then LeakyReLU(out_slope) unless out_slope == 1
  *      act 0: LeakyReLU(slope) (1: none, 0: ReLU); act 1: SiLU.  w, b fp32, each nullable (w_off + w = 1, b = 0): rows of C floats
  *      aff_stride floats apart, one per sample (0: one row for all).  res (nullable): of y's shape; res_w > 0: [N][H/2][res_w/2][C], read
- *      through the nearest x2 upsample (res_w = full width; even height and width).  mean, rstd [N][G] are written for the backward.
- *      ws >= m355_group_norm_ws_bytes(.., 0) bytes, 16-byte aligned; 0 = bad sizes.  A group of more channels than 256 vectors of at most
- *      16 bytes hold is M355_ERR_UNSUPPORTED.  Nothing is launched for N == 0 or HW == 0.
- *      _bwd: dy -> dx (nullable), dw / db (nullable; per_sample: [N][C], else [C] summed over the samples; overwritten), res_w as
- *      in the forward, dres (nullable: 2 x 2 sums of dy, [N][H/2][res_w/2][C]).  The derivative of out_slope is the caller's (as m355_affine_act_fwd). */
-size_t m355_group_norm_ws_bytes(long long N, long long HW, int C, int G, int dtype, int backward);
-int m355_group_norm_fwd(const void *x, const float *w, const float *b, long long aff_stride, float w_off, const void *res, int res_w,
-                        void *y, float *mean, float *rstd, void *ws, long long N, long long HW, int C, int G, float eps, int act,
-                        float slope, float out_slope, int dtype, void *stream);
-int m355_group_norm_bwd(const void *dy, const void *x, const float *w, const float *b, long long aff_stride, float w_off,
-                        const float *mean, const float *rstd, void *dx, float *dw, float *db, int per_sample, void *dres, int res_w,
-                        void *ws, long long N, long long HW, int C, int G, int act, float slope, int dtype, void *stream);
+ *      through the nearest x2 upsample (res_w = full width; even height and width).  stat [2][N][G] floats: mean and rstd, for the backward.
+ *      ws >= m355_group_norm_ws_bytes(d, 0) bytes, 16-byte aligned; 0 = bad sizes.  Groups of more channels than 256 vectors hold (of 16
+ *      bytes, or what the channel count and the addresses are multiples of) are M355_ERR_UNSUPPORTED.  Nothing is launched for an empty x.
+ *      _bwd: dy -> dx (nullable), dw / db (nullable; per_sample: [N][C], else [C] summed over the samples; overwritten), dres (nullable,
+ *      res_w > 0: 2 x 2 sums of dy, [N][H/2][res_w/2][C]).  The derivative of out_slope is the caller's (as m355_affine_act_fwd). */
+typedef struct {
+    long long N, HW, aff_stride;
+    int C, G, dtype, act, res_w, per_sample;
+    float eps, slope, out_slope, w_off;
+} m355_gn_desc;
+size_t m355_group_norm_ws_bytes(const m355_gn_desc *d, int backward);
+int m355_group_norm_fwd(const m355_gn_desc *d, const void *x, const float *w, const float *b, const void *res, void *y, float *stat, void *ws,
+                        void *stream);
+int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const void *x, const float *w, const float *b, const float *stat, void *dx,
+                        float *dw, float *db, void *dres, void *ws, void *stream);
 
 /* ---- Global norm of a list of gradients, and clipping by it.  in / out / numel / dtype: HOST arrays of n entries (device pointers,
  *      element counts, m355_dtype).  norm (device, 1 float) = |scale| sqrt(sum of squares, added in 64 bits in a fixed order);

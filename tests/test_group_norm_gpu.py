@@ -124,6 +124,10 @@ CASES = [
     ((1, 4, 3, 1030), 10, H, "silu", 1.0, "sample", "full"),    # slabs of vectors of two over groups of 103, the last one short
     ((2, 3, 3, 520), 4, F, "lrelu", 0.2, "layer", "none"),
     ((1, 2, 2, 2048), 1, BF, "silu", 1.0, "layer", "none"),     # the widest group of a 16-bit type
+    ((1, 16, 16, 1024), 32, BF, "lrelu", 0.2, "sample", "half"),   # one pass, rows of 64 bytes
+    ((40, 16, 16, 1024), 32, BF, "lrelu", 0.2, "layer", "half"),   # one pass, rows of 128 bytes, 8 vectors a thread
+    ((2, 32, 16, 256), 32, BF, "silu", 1.0, "layer", "full"),      # one pass, rows of 64 bytes, 8 vectors a thread
+    ((2, 31, 17, 96), 3, H, "lrelu", 0.2, "layer", "none"),        # a slab of a whole group of 32
     ((257, 2, 1, 16), 2, BF, "lrelu", 0.2, "sample", "none"),   # many samples
     ((1, 300, 301, 6), 3, BF, "lrelu", 0.2, "layer", "none"),   # many ranges, the last one short
     ((1, 258, 130, 16), 2, F, "silu", 1.0, "layer", "half"),

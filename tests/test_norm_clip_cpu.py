@@ -34,34 +34,38 @@ def test_cpu_tensors_are_refused(pkg):
 FAKE = ctypes.c_void_p(0x10000)     # device pointers are only looked at
 
 
-def _fwd(L, n=2, hw=16, c=8, g=2, dtype=2, act=0, res=None, res_w=0, x=FAKE, y=ctypes.c_void_p(0x20000), ws=FAKE):
-    return L.m355_group_norm_fwd(x, None, None, 0, 0.0, res, res_w, y, FAKE, FAKE, ws, n, hw, c, g, 1e-5, act, 0.2, 1.0, dtype, None)
+def _desc(pkg, n=2, hw=16, c=8, g=2, dtype=2, act=0, res_w=0, stride=0, per_sample=0):
+    return ctypes.byref(pkg._lib.GnDesc(n, hw, stride, c, g, dtype, act, res_w, per_sample, 1e-5, 0.2, 1.0, 0.0))
 
 
-def _bwd(L, n=2, hw=16, c=8, g=2, dtype=2, act=0, dres=None, res_w=0, dy=FAKE, dx=ctypes.c_void_p(0x20000)):
-    return L.m355_group_norm_bwd(dy, ctypes.c_void_p(0x30000), None, None, 0, 0.0, FAKE, FAKE, dx, None, None, 0, dres, res_w, FAKE, n, hw, c,
-                                 g, act, 0.2, dtype, None)
+def _fwd(pkg, res=None, x=FAKE, y=ctypes.c_void_p(0x20000), ws=FAKE, **kw):
+    return pkg._lib.lib().m355_group_norm_fwd(_desc(pkg, **kw), x, None, None, res, y, FAKE, ws, None)
+
+
+def _bwd(pkg, dres=None, dy=FAKE, dx=ctypes.c_void_p(0x20000), **kw):
+    return pkg._lib.lib().m355_group_norm_bwd(_desc(pkg, **kw), dy, ctypes.c_void_p(0x30000), None, None, FAKE, dx, None, None, dres, FAKE, None)
 
 
 def test_group_norm_entry_points_check_their_arguments(pkg):
     L = pkg._lib.lib()
     for kw in (dict(n=-1), dict(hw=-1), dict(c=0), dict(g=0), dict(g=3), dict(dtype=3), dict(dtype=-1), dict(act=2), dict(n=1 << 31),
-               dict(hw=1 << 40)):
-        assert _fwd(L, **kw) == -1 and L.m355_last_error()
-        assert _bwd(L, **kw) == -1 and L.m355_last_error()
-    assert _fwd(L, x=None) == -1 and b"null" in L.m355_last_error()
-    assert _fwd(L, ws=None) == -1 and _fwd(L, y=FAKE) == -1
-    assert _fwd(L, res=FAKE, res_w=3) == -1 and _fwd(L, res=FAKE, res_w=-2) == -1 and _fwd(L, res=None, res_w=4) == -1
-    assert _fwd(L, res=FAKE, res_w=16, hw=16) == -1                    # one row: no half height
-    assert _bwd(L, dres=FAKE, res_w=0) == -1 and _bwd(L, dres=FAKE, res_w=16, hw=16) == -1
-    assert _bwd(L, dy=None) == -1 and _bwd(L, dx=FAKE) == -1
+               dict(hw=1 << 40), dict(c=1 << 21, g=1 << 20), dict(stride=-1), dict(res_w=3), dict(res_w=-2),
+               dict(res_w=16)):                                        # (one row: no half height)
+        assert _fwd(pkg, res=FAKE, **kw) == -1 and L.m355_last_error()
+        assert _bwd(pkg, dres=FAKE, **kw) == -1 and L.m355_last_error()
+        assert L.m355_group_norm_ws_bytes(_desc(pkg, **kw), 1) == 0
+    assert L.m355_group_norm_fwd(None, FAKE, None, None, None, FAKE, FAKE, FAKE, None) == -1
+    assert _fwd(pkg, x=None) == -1 and b"null" in L.m355_last_error()
+    assert _fwd(pkg, ws=None) == -1 and _fwd(pkg, y=FAKE) == -1
+    assert _fwd(pkg, res=None, res_w=4) == -1
+    assert _bwd(pkg, dres=FAKE, res_w=0) == -1
+    assert _bwd(pkg, dy=None) == -1 and _bwd(pkg, dx=FAKE) == -1
     # a group wider than a workgroup: 257 odd channels, 4096 of a vector of eight
     for c, g, dtype in ((257, 1, 2), (771, 3, 0), (4096, 1, 2), (2056, 1, 2)):
-        assert _fwd(L, c=c, g=g, dtype=dtype) == -2 and _bwd(L, c=c, g=g, dtype=dtype) == -2
+        assert _fwd(pkg, c=c, g=g, dtype=dtype) == -2 and _bwd(pkg, c=c, g=g, dtype=dtype) == -2
     # nothing to do is no error, and launches nothing
-    assert _fwd(L, n=0) == 0 and _fwd(L, hw=0) == 0 and _bwd(L, n=0) == 0 and _bwd(L, hw=0) == 0
-    assert L.m355_group_norm_ws_bytes(2, 16, 8, 3, 2, 0) == 0
-    small, back = L.m355_group_norm_ws_bytes(2, 16, 8, 2, 2, 0), L.m355_group_norm_ws_bytes(2, 16, 8, 2, 2, 1)
+    assert _fwd(pkg, n=0) == 0 and _fwd(pkg, hw=0) == 0 and _bwd(pkg, n=0) == 0 and _bwd(pkg, hw=0) == 0
+    small, back = L.m355_group_norm_ws_bytes(_desc(pkg), 0), L.m355_group_norm_ws_bytes(_desc(pkg), 1)
     assert small >= 2 * 2 * 8 and back >= small + 2 * 2 * 8 * 4
 
 
