@@ -18,7 +18,8 @@ namespace gc {
 constexpr int kT = 256;
 constexpr int kMaxT = 112;           // tensors a launch: 3.3 KB of kernel arguments (4 KB is the limit)
 constexpr int kGrid = 1024;          // workgroups (= partial sums) a launch at most
-constexpr int kChunk = 8192;         // values of a piece of work
+constexpr int kU = 8;                // 16-byte vectors a thread has in flight
+constexpr int kPiece = 32768;        // bytes of a piece of work: kU vectors of every thread
 
 struct Table {
     const void *in[kMaxT];
@@ -27,6 +28,7 @@ struct Table {
     unsigned start[kMaxT + 1];       // first piece of each tensor
     unsigned char dtype[kMaxT];
     int count;
+    unsigned per;                    // pieces a workgroup, one behind the other
 };
 
 __device__ __forceinline__ double block_sum(double v, double *s)
@@ -55,39 +57,82 @@ template <typename T, int V> struct Any {
     typedef T vt __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 
-template <typename T> __device__ __forceinline__ double piece_square(const T *p, int n)
+// a vector at any element's address; NT: past the memory-side cache
+template <bool NT, typename T> __device__ __forceinline__ typename Any<T, 16 / sizeof(T)>::vt get(const T *p)
 {
-    constexpr int V = 16 / sizeof(T);
-    double acc = 0.0;
-    int i = (int)threadIdx.x * V;
-    for (; i + V <= n; i += kT * V) {
-        const typename Any<T, V>::vt v = *reinterpret_cast<const typename Any<T, V>::vt *>(p + i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const double d = (double)(float)v[j];
-            acc += d * d;
-        }
-    }
-    for (int k = 0; k < V && i + k < n; ++k) {
-        const double d = (double)(float)p[i + k];
-        acc += d * d;
-    }
-    return acc;
+    typedef typename Any<T, 16 / sizeof(T)>::vt vt;
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const vt *>(p));
+    else return *reinterpret_cast<const vt *>(p);
+}
+template <bool NT, typename T> __device__ __forceinline__ void put(T *p, const typename Any<T, 16 / sizeof(T)>::vt &v)
+{
+    typedef typename Any<T, 16 / sizeof(T)>::vt vt;
+    if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<vt *>(p));
+    else *reinterpret_cast<vt *>(p) = v;
 }
 
-__global__ __launch_bounds__(kT) void k_grad_square(const Table t, double *__restrict__ part)
+// f(offset, vector) over a piece of n values, one(offset) over those behind the last vector
+template <bool NT, typename T, typename F, typename G> __device__ __forceinline__ void walk(const T *p, int n, F f, G one)
+{
+    constexpr int V = 16 / sizeof(T);
+    typedef typename Any<T, V>::vt vt;
+    int i = (int)threadIdx.x * V;
+    if (n == kPiece / (int)sizeof(T)) {
+        vt v[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) v[u] = get<NT>(p + i + u * kT * V);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) f(i + u * kT * V, v[u]);
+        return;
+    }
+    for (; i + V <= n; i += kT * V) f(i, get<false>(p + i));
+    for (int k = 0; k < V && i + k < n; ++k) one(i + k);
+}
+
+// f(tensor, first value, values) over the workgroup's pieces
+template <typename F> __device__ __forceinline__ void pieces_of(const Table &t, F f)
+{
+    const unsigned all = t.start[t.count];
+    unsigned k = blockIdx.x * t.per;
+    const unsigned end = min(all, k + t.per);
+    if (k >= end) return;
+    for (int i = tensor_of(t, k); k < end; ++k) {
+        while (k >= t.start[i + 1]) ++i;   // (every tensor of the table has a piece)
+        const long long len = t.dtype[i] == M355_F32 ? kPiece / 4 : kPiece / 2, o = (long long)(k - t.start[i]) * len;
+        f(i, o, (int)min(len, t.n[i] - o));
+    }
+}
+
+template <bool NT, typename T> __device__ __forceinline__ double piece_square(const T *p, int n)
+{
+    constexpr int V = 16 / sizeof(T);
+    double a0 = 0.0, a1 = 0.0;
+    walk<NT>(
+        p, n,
+        [&](int, const typename Any<T, V>::vt &v) {
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const double d = (double)(float)v[j], e = (double)(float)v[j + 1];
+                a0 += d * d;
+                a1 += e * e;
+            }
+        },
+        [&](int i) {
+            const double d = (double)(float)p[i];
+            a0 += d * d;
+        });
+    return a0 + a1;
+}
+
+template <bool NT> __global__ __launch_bounds__(kT) void k_grad_square(const Table t, double *__restrict__ part)
 {
     __shared__ double s[4];
     double acc = 0.0;
-    const unsigned pieces = t.start[t.count];
-    for (unsigned k = blockIdx.x; k < pieces; k += gridDim.x) {
-        const int i = tensor_of(t, k);
-        const long long o = (long long)(k - t.start[i]) * kChunk;
-        const int n = (int)min((long long)kChunk, t.n[i] - o);
-        if (t.dtype[i] == M355_F32) acc += piece_square((const float *)t.in[i] + o, n);
-        else if (t.dtype[i] == M355_F16) acc += piece_square((const _Float16 *)t.in[i] + o, n);
-        else acc += piece_square((const __bf16 *)t.in[i] + o, n);
-    }
+    pieces_of(t, [&](int i, long long o, int n) {
+        if (t.dtype[i] == M355_F32) acc += piece_square<NT>((const float *)t.in[i] + o, n);
+        else if (t.dtype[i] == M355_F16) acc += piece_square<NT>((const _Float16 *)t.in[i] + o, n);
+        else acc += piece_square<NT>((const __bf16 *)t.in[i] + o, n);
+    });
     const double v = block_sum(acc, s);
     if (threadIdx.x == 0) part[blockIdx.x] = v;
 }
@@ -107,19 +152,21 @@ __global__ __launch_bounds__(kT) void k_grad_norm(const double *__restrict__ par
     if (threadIdx.x == 0) *norm = (float)v;
 }
 
-template <typename T> __device__ __forceinline__ void piece_scale(const T *p, T *q, int n, float c)
+template <bool NT, typename T> __device__ __forceinline__ void piece_scale(const T *p, T *q, int n, float c)
 {
     constexpr int V = 16 / sizeof(T);
-    int i = (int)threadIdx.x * V;
-    for (; i + V <= n; i += kT * V) {
-        typename Any<T, V>::vt v = *reinterpret_cast<const typename Any<T, V>::vt *>(p + i);
+    typedef typename Any<T, V>::vt vt;
+    walk<NT>(
+        p, n,
+        [&](int i, vt v) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = (T)((float)v[j] * c);
-        *reinterpret_cast<typename Any<T, V>::vt *>(q + i) = v;
-    }
-    for (int k = 0; k < V && i + k < n; ++k) q[i + k] = (T)((float)p[i + k] * c);
+            for (int j = 0; j < V; ++j) v[j] = (T)((float)v[j] * c);
+            put<NT>(q + i, v);
+        },
+        [&](int i) { q[i] = (T)((float)p[i] * c); });
 }
 
+template <bool NT>
 __global__ __launch_bounds__(kT) void k_grad_scale(const Table t, const double *__restrict__ part, int nparts, double scale, double max_norm,
                                                    float *__restrict__ norm, int write_norm)
 {
@@ -129,16 +176,12 @@ __global__ __launch_bounds__(kT) void k_grad_scale(const Table t, const double *
     // (a NaN norm fails the comparison: every gradient becomes NaN; an infinite one makes the factor 0)
     const double q = isinf(max_norm) ? 1.0 : max_norm / (v + 1e-6);   // (an infinite threshold never clips)
     const float c = (float)(scale * (q >= 1.0 ? 1.0 : q));
-    const unsigned pieces = t.start[t.count];
-    for (unsigned k = blockIdx.x; k < pieces; k += gridDim.x) {
-        const int i = tensor_of(t, k);
-        const long long o = (long long)(k - t.start[i]) * kChunk;
-        const int n = (int)min((long long)kChunk, t.n[i] - o);
-        if (c == 1.0f && t.in[i] == t.out[i]) continue;   // (times one in place)
-        if (t.dtype[i] == M355_F32) piece_scale((const float *)t.in[i] + o, (float *)t.out[i] + o, n, c);
-        else if (t.dtype[i] == M355_F16) piece_scale((const _Float16 *)t.in[i] + o, (_Float16 *)t.out[i] + o, n, c);
-        else piece_scale((const __bf16 *)t.in[i] + o, (__bf16 *)t.out[i] + o, n, c);
-    }
+    pieces_of(t, [&](int i, long long o, int n) {
+        if (c == 1.0f && t.in[i] == t.out[i]) return;   // (times one in place)
+        if (t.dtype[i] == M355_F32) piece_scale<NT>((const float *)t.in[i] + o, (float *)t.out[i] + o, n, c);
+        else if (t.dtype[i] == M355_F16) piece_scale<NT>((const _Float16 *)t.in[i] + o, (_Float16 *)t.out[i] + o, n, c);
+        else piece_scale<NT>((const __bf16 *)t.in[i] + o, (__bf16 *)t.out[i] + o, n, c);
+    });
 }
 
 struct Span {
@@ -147,6 +190,12 @@ struct Span {
 };
 
 static inline int esize(int dtype) { return dtype == M355_F32 ? 4 : 2; }
+
+static inline unsigned long long pieces(long long numel, int dtype)
+{
+    const long long len = kPiece / esize(dtype);
+    return (unsigned long long)((numel + len - 1) / len);
+}
 
 // no output may share memory with another output, or with another tensor's input
 static int check_overlap(const void *const *in, void *const *out, const long long *numel, const int *dtype, int n)
@@ -204,13 +253,14 @@ extern "C" int m355_grad_clip(const void *const *in, void *const *out, const lon
         M355_REQUIRE(numel[i] == 0 || (in[i] && (!out || out[i])), "grad_clip: tensor %d is null", i);
         M355_REQUIRE(((uintptr_t)in[i] % gc::esize(dtype[i])) == 0 && (!out || ((uintptr_t)out[i] % gc::esize(dtype[i])) == 0),
                      "grad_clip: tensor %d is not aligned to its element", i);
-        total += (unsigned long long)(numel[i] + gc::kChunk - 1) / gc::kChunk;
+        total += gc::pieces(numel[i], dtype[i]);
         M355_REQUIRE(total < (1ULL << 32), "grad_clip: the list is too large");
     }
     if (out && n > 0) {
         const int rc = gc::check_overlap(in, out, numel, dtype, n);
         if (rc != M355_OK) return rc;
     }
+    const bool nt = total * gc::kPiece >= (160ULL << 20);   // (more than the memory-side cache keeps between the passes)
     hipStream_t s = (hipStream_t)stream;
     double *part = (double *)ws;
     int nparts = 0;
@@ -222,7 +272,7 @@ extern "C" int m355_grad_clip(const void *const *in, void *const *out, const lon
             unsigned long long pieces = 0;
             for (; i < n && t.count < gc::kMaxT; ++i) {
                 if (numel[i] == 0) continue;
-                const unsigned long long k = (unsigned long long)(numel[i] + gc::kChunk - 1) / gc::kChunk;
+                const unsigned long long k = gc::pieces(numel[i], dtype[i]);
                 t.in[t.count] = in[i];
                 t.out[t.count] = out ? out[i] : nullptr;
                 t.n[t.count] = numel[i];
@@ -232,15 +282,19 @@ extern "C" int m355_grad_clip(const void *const *in, void *const *out, const lon
                 ++t.count;
             }
             t.start[t.count] = (unsigned)pieces;
-            const unsigned grid = (unsigned)std::min<unsigned long long>(pieces, gc::kGrid);
+            unsigned grid = (unsigned)std::min<unsigned long long>(pieces, gc::kGrid);
+            t.per = grid > 0 ? (unsigned)((pieces + grid - 1) / grid) : 1;
+            if (grid > 0) grid = (unsigned)((pieces + t.per - 1) / t.per);
             if (pass == 0) {
                 if (grid > 0) {
-                    hipLaunchKernelGGL(gc::k_grad_square, dim3(grid), dim3(gc::kT), 0, s, t, part + nparts);
+                    if (nt && !out) hipLaunchKernelGGL(gc::k_grad_square<true>, dim3(grid), dim3(gc::kT), 0, s, t, part + nparts);
+                    else hipLaunchKernelGGL(gc::k_grad_square<false>, dim3(grid), dim3(gc::kT), 0, s, t, part + nparts);
                     nparts += (int)grid;
                 }
             } else if (grid > 0 || first) {   // (an empty list still has a norm: 0)
-                hipLaunchKernelGGL(gc::k_grad_scale, dim3(grid > 0 ? grid : 1), dim3(gc::kT), 0, s, t, part, nparts, scale, max_norm, norm,
-                                   first ? 1 : 0);
+                const dim3 g(grid > 0 ? grid : 1);
+                if (nt) hipLaunchKernelGGL(gc::k_grad_scale<true>, g, dim3(gc::kT), 0, s, t, part, nparts, scale, max_norm, norm, first ? 1 : 0);
+                else hipLaunchKernelGGL(gc::k_grad_scale<false>, g, dim3(gc::kT), 0, s, t, part, nparts, scale, max_norm, norm, first ? 1 : 0);
                 first = false;
             }
         }

@@ -27,9 +27,25 @@ def _flat(t):
 
 
 def _check(tensors, what):
-    """-> the list, its device's index, and whether every tensor's values lie together"""
+    """-> the list, its device's index, whether every tensor's values lie together, and the lists of addresses, counts and types"""
     ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    index, together = None, True
+    if not ts:
+        raise ValueError(f"{what}: no gradients")
+    together, at, nums, kinds = True, [], [], []
+    try:
+        index = ts[0].get_device()
+        for t in ts:
+            if t.get_device() != index or index < 0 or t.layout is not _strided:
+                break
+            kinds.append(_DTYPES[t.dtype])
+            nums.append(t.numel())
+            at.append(t.data_ptr())
+            if together and not t.is_contiguous():
+                together = _flat(t) or t.numel() == 0
+        else:
+            return ts, index, together, at, nums, kinds
+    except (AttributeError, KeyError, RuntimeError, NotImplementedError):   # (not tensors, or not of this kind: said below)
+        pass
     for t in ts:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise _lib.M355Error(f"{what}: gradients must be CUDA(HIP) tensors; there is no CPU implementation")
@@ -37,28 +53,20 @@ def _check(tensors, what):
             raise TypeError(f"{what}: a gradient is {t.layout}: dense tensors only")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{what}: gradients must be float32, float16 or bfloat16, got {t.dtype}")
-        d = t.get_device()
-        if d != index:
-            if index is not None:
-                raise ValueError(f"{what}: gradients on cuda:{index} and on {t.device}: clip each device's own list")
-            index = d
-        if together and not t.is_contiguous():
-            together = _flat(t) or t.numel() == 0
-    if not ts:
-        raise ValueError(f"{what}: no gradients")
-    return ts, index, together
+        if t.device != ts[0].device:
+            raise ValueError(f"{what}: gradients on {ts[0].device} and on {t.device}: clip each device's own list")
+    raise _lib.M355Error(f"{what}: a gradient has no memory of its own ({type(ts[0])})")
 
 
-def _run(ts, outs, index, max_norm, scale):
-    n = len(ts)
+def _run(dev, index, at, out, nums, kinds, max_norm, scale):
+    n = len(at)
     with on_device(index):
-        dev = ts[0].device
         ws = torch.empty((lib().m355_grad_clip_ws_bytes(n),), dtype=torch.uint8, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        ptrs = array("Q", [t.data_ptr() for t in ts])
-        optr = None if outs is None else ptrs if outs is ts else array("Q", [t.data_ptr() for t in outs])
-        nums, kinds = array("q", [t.numel() for t in ts]), array("i", [_DTYPES[t.dtype] for t in ts])
-        launch("grad_clip", ptrs.buffer_info()[0], None if outs is None else optr.buffer_info()[0], nums.buffer_info()[0],
+        ptrs = array("Q", at)
+        optr = ptrs if out is at or out is None else array("Q", out)
+        nums, kinds = array("q", nums), array("i", kinds)
+        launch("grad_clip", ptrs.buffer_info()[0], None if out is None else optr.buffer_info()[0], nums.buffer_info()[0],
                kinds.buffer_info()[0], n, scale, max_norm, norm.data_ptr(), ws.data_ptr(), stream())
     return norm
 
@@ -66,11 +74,12 @@ def _run(ts, outs, index, max_norm, scale):
 def grad_norm(grads, scale=1.0):
     """The 2-norm of all values of `grads` (a tensor or an iterable of tensors, float32 / float16 / bfloat16 mixed, one device), times
     |scale|: a 0-dimensional float32 tensor on their device.  Squares are added in 64 bits in a fixed order."""
-    ts, index, together = _check(grads, "grad_norm")
+    ts, index, together, at, nums, kinds = _check(grads, "grad_norm")
     if not together:
         with torch.no_grad():
             ts = [t.contiguous() for t in ts]
-    return _run(ts, None, index, 0.0, float(scale))
+        at = [t.data_ptr() for t in ts]
+    return _run(ts[0].device, index, at, None, nums, kinds, 0.0, float(scale))
 
 
 def clip_grads_(grads, max_norm, out=None, scale=1.0):
@@ -83,19 +92,18 @@ def clip_grads_(grads, max_norm, out=None, scale=1.0):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads_: max_norm={max_norm!r}")
-    ts, index, together = _check(grads, "clip_grads_")
+    ts, index, together, at, nums, kinds = _check(grads, "clip_grads_")
     if not together:
         raise ValueError("clip_grads_: a gradient's values have gaps or repeats between them (an expanded or sliced view)")
-    outs = ts
+    outs, to = ts, at
     if out is not None:
-        outs, o_index, _ = _check(out, "clip_grads_")
-        if len(outs) != len(ts) or o_index != index:
-            raise ValueError(f"clip_grads_: {len(ts)} gradients on cuda:{index}, {len(outs)} outputs on cuda:{o_index}")
+        outs, o_index, together, to, o_nums, o_kinds = _check(out, "clip_grads_")
+        if o_index != index or o_nums != nums or o_kinds != kinds:
+            raise ValueError("clip_grads_: as many outputs as gradients, of their types and shapes, on their device")
         for t, o in zip(ts, outs):
-            if o.dtype is not t.dtype or o.shape != t.shape or (
-                    not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride()):
-                raise ValueError("clip_grads_: an output must have its gradient's type, shape and strides")
-    norm = _run(ts, outs, index, max_norm, float(scale))
+            if not (o.is_same_size(t) and (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride())):
+                raise ValueError("clip_grads_: an output must have its gradient's shape and strides")
+    norm = _run(ts[0].device, index, at, to, nums, kinds, max_norm, float(scale))
     torch.autograd.graph.increment_version(outs)
     return norm
 
