@@ -15,6 +15,7 @@ import torch.nn.functional as F
 
 from . import conv as C
 from . import gan_ops as G
+from .group_norm import GroupNorm2d, GroupNormAct2d
 
 LRELU = 0.2  # nn.LeakyReLU(0.2) everywhere in models/gan.py
 
@@ -118,6 +119,8 @@ class ConditionalBatchNorm2d(nn.Module):
             self.norm = G.InstanceNorm2d(ch)
         elif args.norm_g == 'none':
             self.norm = G.NoNorm()
+        elif args.norm_g == 'group':   # (not one of the reference's: no batch statistics, for few samples per GPU)
+            self.norm = GroupNorm2d(ch, getattr(args, "norm_groups", 32))
         else:
             raise ValueError(f"norm_g={args.norm_g!r}")
         self.fc_gamma = nn.Linear(emb_dim, ch)
@@ -332,6 +335,8 @@ def _d_norm(args, ch):
         return nn.InstanceNorm2d(ch, affine=True), False
     if args.norm_d == 'none':
         return None, True
+    if args.norm_d == 'group':   # (not one of the reference's: instance norm's place, fused with the LeakyReLU, on NHWC)
+        return GroupNormAct2d(ch, getattr(args, "norm_groups", 32)), False
     raise ValueError(f"norm_d={args.norm_d!r}")
 
 
@@ -394,7 +399,7 @@ class _DiscBase(nn.Module):
         return C.dgrad_mask_ok(C.make_desc(s[0], s[1], s[2], s[3], conv.out_channels, kh, kw, st, ph, pw, mode, 0))
 
     def _act(self, conv, norm, x, in_act=False, sole_consumer_masks=False):
-        """conv -> [InstanceNorm] -> LeakyReLU on NHWC bf16.  With the activation in the conv epilogue (no norm):
+        """conv -> [InstanceNorm | GroupNorm] -> LeakyReLU on NHWC bf16.  With the activation in the conv epilogue (no norm):
         in_act = x is the previous layer's fused conv+LeakyReLU output and this conv is its only consumer -> this
         conv's dgrad applies that activation's backward; sole_consumer_masks = the same arrangement one layer up,
         i.e. this layer's incoming gradient is already masked."""
@@ -402,6 +407,8 @@ class _DiscBase(nn.Module):
             fuse = x.is_cuda and conv.m355[3] != C.PAD_REPLICATE
             return conv(x, slope=LRELU, in_slope=LRELU if (in_act and fuse) else 1.0,
                         premasked=sole_consumer_masks and fuse)
+        if isinstance(norm, GroupNormAct2d):
+            return norm(conv(x), slope=LRELU)
         y = G.to_nchw_f32(conv(x))
         return G.to_nhwc_bf16(F.leaky_relu(norm(y), LRELU))
 

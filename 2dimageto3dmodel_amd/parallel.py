@@ -110,11 +110,28 @@ def grad_group():
     return _GRAD_GROUP[0]
 
 
+def _store_averages(parts, max_norm):
+    """parts: (flat sum over the ranks, parameters, views of the sum shaped as they are).  Writes the averages to the parameters' .grad;
+    max_norm: clipped to that global norm over all parts in the same pass (grad_clip.clip_grads_) -> the norm before clipping"""
+    scale = 1.0 / world_size()
+    if max_norm is not None:
+        from .grad_clip import clip_grads_
+        views = [v for _, _, vs in parts for v in vs]
+        grads = [p.grad for _, ps, _ in parts for p in ps]
+        if all(g.is_contiguous() and g.dtype == torch.float32 for g in grads):
+            return clip_grads_(views, max_norm, out=grads, scale=scale)
+    for flat, ps, views in parts:
+        flat.mul_(scale)
+        torch._foreach_copy_([p.grad for p in ps], views)
+    return None if max_norm is None else clip_grads_([p.grad for _, ps, _ in parts for p in ps], max_norm)
+
+
 class FlatGradReducer:
     """Averages the gradients of `params` over the ranks with one all-reduce of a persistent flat buffer.
     reducer() = start() + finish(); start() issues the collective asynchronously on the gradient group's communicator (the
     compute stream is not blocked), finish() makes the compute stream wait for it and writes the averages back -- the trainer
-    puts the next generator forward between the two (train.GanTrainer: overlap of the discriminator's all-reduce)."""
+    puts the next generator forward between the two (train.GanTrainer: overlap of the discriminator's all-reduce).  finish(max_norm)
+    also clips the averages to that global norm, in the pass that writes them back, and returns the norm."""
 
     def __init__(self, params):
         self.params = [p for p in params if p.requires_grad]
@@ -145,9 +162,14 @@ class FlatGradReducer:
         self._pending = (work, ps, views, ev, t0, n)
         return True
 
-    def finish(self):
+    def finish(self, max_norm=None):
+        part = self._wait()
+        return None if part is None else _store_averages([part], max_norm)
+
+    def _wait(self):
+        """wait for the collective -> (flat sum, parameters, views), None when nothing was started"""
         if self._pending is None:
-            return
+            return None
         work, ps, views, ev, t0, n = self._pending
         self._pending = None
         timed = stats["time_allreduce"]
@@ -174,12 +196,11 @@ class FlatGradReducer:
             stats["wait_events"].append((now - tw) * 1e3)
         stats["grad_allreduces"] += 1
         stats["grad_allreduce_bytes"] += 4 * n
-        self.flat.mul_(1.0 / world_size())
-        torch._foreach_copy_([p.grad for p in ps], views)
+        return self.flat, ps, views
 
-    def __call__(self):
-        if self.start():
-            self.finish()
+    def __call__(self, max_norm=None):
+        """-> the norm before clipping (max_norm given), None when there was nothing to reduce: the caller clips"""
+        return self.finish(max_norm) if self.start() else None
 
 
 # ------------------------------------------------------------------------------------------------ SyncBN messages without RCCL
@@ -320,16 +341,22 @@ class BucketedGradReducer:
             any_ = self.start_bucket(k) or any_
         return any_
 
-    def finish(self):
-        for k, r in enumerate(self.reducers):
-            r.finish()
-            self.started[k] = False
-
-    def __call__(self):
-        if self.start():
-            self.finish()
-        else:
+    def finish(self, max_norm=None):
+        """max_norm: ONE norm over all buckets"""
+        if max_norm is None:
+            for r in self.reducers:
+                r.finish()
             self.started = [False] * len(self.reducers)
+            return None
+        parts = [p for p in (r._wait() for r in self.reducers) if p is not None]
+        self.started = [False] * len(self.reducers)
+        return _store_averages(parts, max_norm) if parts else None
+
+    def __call__(self, max_norm=None):
+        if self.start():
+            return self.finish(max_norm)
+        self.started = [False] * len(self.reducers)
+        return None
 
 
 # ------------------------------------------------------------------------------------------------ projection path

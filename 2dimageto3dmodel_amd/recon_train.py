@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from . import mesh as M
 from . import parallel as P
+from .grad_clip import clip_grad_norm_
 from .reconstruction import BatchNorm1d, BatchNormAct2d, DatasetParams, ReconstructionNetwork
 from .render import Renderer
 
@@ -63,16 +64,21 @@ class ReconTrainer(nn.Module):
         DatasetParams' gradients per iteration (parallel.FlatGradReducer) gives the global-batch gradient -- the per-image rows of
         the DatasetParams table a rank did not touch contribute zeros, as they do in the single-GPU step;
       * parameters are broadcast from rank 0 once; the optimisers then stay in lock step (identical gradients, identical state).
-    tests/test_distributed_gpu.py runs two ranks against the single-process step on the concatenated batch."""
+    tests/test_distributed_gpu.py runs two ranks against the single-process step on the concatenated batch.
+
+    Not the reference's, off by default: norm='group' (ReconstructionNetwork: group norm for batch norm), and max_grad_norm -- the
+    network's gradients are clipped to that global norm (of the averaged gradients) before its optimiser step; the norm before clipping
+    is `grad_norm` of the returned dict, a device scalar."""
 
     def __init__(self, mesh_template, dataset_size=None, symmetric=True, texture_resolution=128, mesh_resolution=32,
                  image_resolution=256, loss='mse', lr=1e-4, lr_dataset=1e-4, mesh_regularization=0.00005, optimize_deltas=True,
-                 optimize_z0=False, interpolation_mode='nearest', device='cuda', data_parallel=True, sync_bn=True):
+                 optimize_z0=False, interpolation_mode='nearest', device='cuda', data_parallel=True, sync_bn=True, norm='batch',
+                 norm_groups=32, max_grad_norm=None):
         super().__init__()
         import argparse
         self.mesh_template = mesh_template
         self.generator = ReconstructionNetwork(symmetric=symmetric, texture_res=texture_resolution, mesh_res=mesh_resolution,
-                                               interpolation_mode=interpolation_mode)
+                                               interpolation_mode=interpolation_mode, norm=norm, norm_groups=norm_groups)
         self.renderer = Renderer(image_resolution, image_resolution)   # (:86-89: the network's input resolution)
         self.optimize_deltas, self.optimize_z0 = bool(optimize_deltas), bool(optimize_z0)
         self.dataset_params = None
@@ -99,6 +105,7 @@ class ReconTrainer(nn.Module):
         self.optimizer = torch.optim.Adam(self.generator.parameters(), lr=lr)
         self.optimizer_dataset = None if self.dataset_params is None else torch.optim.Adam(self.dataset_params.parameters(),
                                                                                            lr=lr_dataset)
+        self.max_grad_norm = max_grad_norm
         self.total_it = 0
 
     def render(self, X_real, gt_scale, gt_translation, gt_rot, gt_idx=None):
@@ -133,11 +140,15 @@ class ReconTrainer(nn.Module):
         total.backward()
         if self.reduce is not None:
             self.reduce()          # (no-op unless more than one rank: the gradients become the global-batch means)
+        norm = None if self.max_grad_norm is None else clip_grad_norm_(self.generator.parameters(), self.max_grad_norm)
         self.optimizer.step()
         if self.optimizer_dataset is not None:
             self.optimizer_dataset.step()
         self.total_it += 1
-        return {"loss": total.detach(), "recon_loss": recon_loss.detach(), "flat_loss": flat_loss.detach(), "miou": miou}
+        out = {"loss": total.detach(), "recon_loss": recon_loss.detach(), "flat_loss": flat_loss.detach(), "miou": miou}
+        if norm is not None:
+            out["grad_norm"] = norm
+        return out
 
     def decay_lr(self, factor=0.5):
         """the halving every `lr_decay_every` epochs (:468-470) -- the generator's optimiser only, as the script"""

@@ -11,6 +11,8 @@ execution, not of meaning:
   * stride-2 5x5 / 3x3 encoder convs: forward on the generic implicit-GEMM kernel, dgrad through the padded even kernel.
 interpolation_mode='bilinear' (:43-44, non-default): the x2 upsample cannot be folded into a conv loader (it mixes four
 pixels); it runs between the blocks as F.interpolate on the NHWC bf16 activation, everything else is unchanged.
+norm='group' (not one of the reference's; default 'batch'): GroupNormAct2d in the place of every batch norm, the two fully connected
+layers' included -- the network then has no batch statistics, and its parameter names stay.
 `DatasetParams` (:140-180): the per-image translation / scale / z0 offsets run_reconstruction.py optimises next to the network.
 """
 import torch
@@ -19,6 +21,7 @@ import torch.nn as nn
 from . import conv as C
 from . import gan_ops as G
 from .gan import Conv2d, _Identity, adjust_poles, symmetrize_texture
+from .group_norm import GroupNormAct2d
 
 
 class BatchNormAct2d(G.BatchNorm2d):
@@ -67,12 +70,12 @@ class BatchNorm1d(nn.BatchNorm1d):
 class ResBlock(nn.Module):
     """models/reconstruction.py:7-26"""
 
-    def __init__(self, ch_in, ch_out, pad_mode):
+    def __init__(self, ch_in, ch_out, pad_mode, norm=BatchNormAct2d):
         super().__init__()
         self.conv1 = Conv2d(ch_in, ch_in, 3, pad_h=1, pad_w=1, pad_w_mode=pad_mode, bias=False)
         self.conv2 = Conv2d(ch_in, ch_out, 3, pad_h=1, pad_w=1, pad_w_mode=pad_mode, bias=False)
-        self.bn1 = BatchNormAct2d(ch_in)
-        self.bn2 = BatchNormAct2d(ch_out)
+        self.bn1 = norm(ch_in)
+        self.bn2 = norm(ch_out)
         if ch_in != ch_out:
             self.shortcut = Conv2d(ch_in, ch_out, 1, bias=False)
         else:
@@ -129,8 +132,12 @@ class DatasetParams(nn.Module):
 class ReconstructionNetwork(nn.Module):
     """models/reconstruction.py:28-137"""
 
-    def __init__(self, symmetric=True, texture_res=64, mesh_res=32, interpolation_mode='nearest'):
+    def __init__(self, symmetric=True, texture_res=64, mesh_res=32, interpolation_mode='nearest', norm='batch', norm_groups=32):
         super().__init__()
+        if norm not in ('batch', 'group'):
+            raise ValueError(f"norm={norm!r}")
+        norm2d = BatchNormAct2d if norm == 'batch' else (lambda ch: GroupNormAct2d(ch, norm_groups))
+        norm1d = BatchNorm1d if norm == 'batch' else norm2d
         self.symmetric = symmetric
         self.pad = C.PAD_REPLICATE if symmetric else C.PAD_CIRCULAR   # (:34-37)
         if interpolation_mode not in ('nearest', 'bilinear'):
@@ -141,42 +148,42 @@ class ReconstructionNetwork(nn.Module):
 
         # encoder: five stride-2 convolutions halve 256 x 256 down to 8 x 8 (:53-63)
         self.conv1e = Conv2d(4, 64, 5, stride=2, pad_h=2, pad_w=2, bias=False)
-        self.bn1e = BatchNormAct2d(64)
+        self.bn1e = norm2d(64)
         self.conv2e = Conv2d(64, 128, 3, stride=2, pad_h=1, pad_w=1, bias=False)
-        self.bn2e = BatchNormAct2d(128)
+        self.bn2e = norm2d(128)
         self.conv3e = Conv2d(128, 256, 3, stride=2, pad_h=1, pad_w=1, bias=False)
-        self.bn3e = BatchNormAct2d(256)
+        self.bn3e = norm2d(256)
         self.conv4e = Conv2d(256, 512, 3, stride=2, pad_h=1, pad_w=1, bias=False)
-        self.bn4e = BatchNormAct2d(512)
+        self.bn4e = norm2d(512)
 
         bottleneck_dim = 256
         self.conv5e = Conv2d(512, 64, 3, stride=2, pad_h=1, pad_w=1, bias=False)
-        self.bn5e = BatchNormAct2d(64)
+        self.bn5e = norm2d(64)
         self.fc1e = nn.Linear(64 * 8 * 8, bottleneck_dim, bias=False)
-        self.bnfc1e = BatchNorm1d(bottleneck_dim)
+        self.bnfc1e = norm1d(bottleneck_dim)
         self.fc3e = nn.Linear(bottleneck_dim, 1024, bias=False)
-        self.bnfc3e = BatchNorm1d(1024)
+        self.bnfc3e = norm1d(1024)
 
         # texture decoder: 4 x (2|4) seed, one x2 upsample after every block but the last (:72-90); texture_res 128 / 256
         # insert one / two more 256-channel blocks
         self.base_res_h = 4
         self.base_res_w = 2 if symmetric else 4
         self.fc1_tex = nn.Linear(1024, self.base_res_h * self.base_res_w * 256)
-        self.blk1 = ResBlock(256, 512, self.pad)
-        self.blk2 = ResBlock(512, 256, self.pad)
-        self.blk3 = ResBlock(256, 256, self.pad)
+        self.blk1 = ResBlock(256, 512, self.pad, norm2d)
+        self.blk2 = ResBlock(512, 256, self.pad, norm2d)
+        self.blk3 = ResBlock(256, 256, self.pad, norm2d)
         assert texture_res in [64, 128, 256]
         self.texture_res = texture_res
         if texture_res >= 128:
-            self.blk3b_tex = ResBlock(256, 256, self.pad)
+            self.blk3b_tex = ResBlock(256, 256, self.pad, norm2d)
         if texture_res >= 256:
-            self.blk3c_tex = ResBlock(256, 256, self.pad)
-        self.blk4_tex = ResBlock(256, 128, self.pad)
-        self.blk5_tex = ResBlock(128, 64, self.pad)
+            self.blk3c_tex = ResBlock(256, 256, self.pad, norm2d)
+        self.blk4_tex = ResBlock(256, 128, self.pad, norm2d)
+        self.blk5_tex = ResBlock(128, 64, self.pad, norm2d)
         self.conv_tex = Conv2d(64, 3, 5, pad_h=2, pad_w=2, pad_w_mode=self.pad)
 
         # displacement-map decoder branches off at 32 x 32 (:92-99)
-        self.blk4_mesh = ResBlock(256, 64, self.pad)
+        self.blk4_mesh = ResBlock(256, 64, self.pad, norm2d)
         self.conv_mesh = Conv2d(64, 3, 5, pad_h=2, pad_w=2, pad_w_mode=self.pad)
         # zero-initialised mesh output layer for stability (avoids self-intersections, :97-99)
         self.conv_mesh.bias.data[:] = 0
@@ -193,6 +200,8 @@ class ReconstructionNetwork(nn.Module):
     def encode(self, x):
         """image -> bottleneck code z [B,1024] (:108-116)"""
         z = self.encode_convs(x).reshape(x.shape[0], -1)        # flatten in the reference's (C,H,W) order
+        if isinstance(self.bnfc1e, GroupNormAct2d):   # (the ReLU is part of it)
+            return self.bnfc3e(self.fc3e(self.bnfc1e(self.fc1e(z))))
         z = torch.relu(self.bnfc1e(self.fc1e(z)))
         return torch.relu(self.bnfc3e(self.fc3e(z)))
 

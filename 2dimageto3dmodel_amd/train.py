@@ -13,6 +13,7 @@ from . import conv as CV
 from . import gan as G
 from . import gan_ops as O
 from . import parallel as P
+from .grad_clip import clip_grad_norm_
 
 
 def divide_pred(pred):
@@ -43,8 +44,12 @@ _SN_SITES = int(os.environ.get("M355_SN_PREFETCH_SITES", "7"))
 class GanTrainer(torch.nn.Module):
     def __init__(self, args, latent_dim=64, lr_g=1e-4, lr_d=4e-4, d_steps_per_g=2, loss="hinge", device="cuda",
                  symmetric_g=True, use_mesh=True, ema_alpha=0.999, capturable=False, mesh_template=None,
-                 mesh_regularization=0.0001):
+                 mesh_regularization=0.0001, max_grad_norm_g=None, max_grad_norm_d=None):
+        """max_grad_norm_g / max_grad_norm_d (not the reference's; None: off): the network's gradients -- averaged over the ranks -- are
+        clipped to that global norm before its optimiser step.  The norms before clipping of the last steps are `grad_norms['g']` and
+        `grad_norms['d']`, device scalars."""
         super().__init__()
+        self.max_grad_norm_g, self.max_grad_norm_d, self.grad_norms = max_grad_norm_g, max_grad_norm_d, {}
         # main.py:152,697-705: flat_loss = loss_flat(mesh, compute_normals(get_vertex_positions(pred_mesh))) joins the G loss
         self.mesh_template, self.mesh_regularization = (mesh_template if use_mesh else None), mesh_regularization
         self.args, self.latent_dim, self.d_steps_per_g, self.ema_alpha = args, latent_dim, d_steps_per_g, ema_alpha
@@ -144,11 +149,18 @@ class GanTrainer(torch.nn.Module):
         """complete a discriminator step whose gradient all-reduce is still in flight (see overlap_comm)"""
         if self._pending_d:
             self._pending_d = False
-            self.reduce_d.finish()
+            self._clip('d', self.reduce_d.finish(self.max_grad_norm_d))
             self.optimizer_d.step()
             # (total_it already counts the pending step: a multiple of the cycle length = that step closed a cycle, and the forward this
             # prefetch serves belongs to the next one -- not issued inside a hipGraph capture, which must end with every stream joined)
             self._prefetch_sn(self.discriminator, cross_cycle=self.total_it % (1 + self.d_steps_per_g) == 0, site=2)
+
+    def _clip(self, net, norm):
+        """`norm`: what the reducer returned -- the norm if it averaged and clipped in one pass, None if it had nothing to do"""
+        limit = self.max_grad_norm_g if net == 'g' else self.max_grad_norm_d
+        if limit is not None:
+            params = (self.generator if net == 'g' else self.discriminator).parameters()
+            self.grad_norms[net] = clip_grad_norm_(params, limit) if norm is None else norm
 
     # ---- spectral norm ahead of its forward (gan_ops.SpectralNormGroup.prefetch).  A network's power iteration + bf16 weight views
     # depend on its weights and u / v only, so they are issued on a second stream as soon as those are final for the next forward:
@@ -256,7 +268,7 @@ class GanTrainer(torch.nn.Module):
                 self.generator.grad_barrier = None
                 for p in d_params:
                     p.requires_grad_(True)
-            self.reduce_g()
+            self._clip('g', self.reduce_g(self.max_grad_norm_g))
             self.optimizer_g.step()
             self.update_generator_running_avg(epoch)
             out = {"g": loss.detach()}
@@ -271,7 +283,7 @@ class GanTrainer(torch.nn.Module):
             if self.overlap_comm and self.reduce_d.start():
                 self._pending_d = True                     # finished after the next iteration's generator forward
             else:
-                self.reduce_d()
+                self._clip('d', self.reduce_d(self.max_grad_norm_d))
                 self.optimizer_d.step()
                 self._prefetch_sn(self.discriminator, cross_cycle=(self.total_it + 1) % (1 + self.d_steps_per_g) == 0, site=2)
             out = {"d_fake": loss_fake.detach(), "d_real": loss_real.detach()}

@@ -97,6 +97,8 @@ def cbn(w, name, x, z, norm, training):
             n["num_batches_tracked"].add_(1)
     elif norm == "instance":
         x = F.instance_norm(x)
+    elif norm == "group":
+        x = F.group_norm(x, 32)
     gamma = F.linear(z, c["fc_gamma.weight"], c["fc_gamma.bias"])[:, :, None, None]
     beta = F.linear(z, c["fc_beta.weight"], c["fc_beta.bias"])[:, :, None, None]
     return x * (1 + gamma) + beta
@@ -188,6 +190,8 @@ def generator(w, args, z, c=None, caption=None, symmetric=True, training=True):
 def _d_norm(w, name, x, args):
     if args.norm_d == "instance":   # nn.InstanceNorm2d(nc, affine=True), gan.py:29-31,129-131
         return F.instance_norm(x, weight=w[name + ".weight"], bias=w[name + ".bias"])
+    if args.norm_d == "group":
+        return F.group_norm(x, 32, w[name + ".weight"], w[name + ".bias"])
     return x
 
 

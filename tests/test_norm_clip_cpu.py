@@ -93,3 +93,25 @@ def test_clip_entry_point_checks_its_arguments(pkg):
         assert _clip(L, ins, outs, **ok) == -1 and b"shares memory" in L.m355_last_error(), (ins, outs)
     assert L.m355_grad_clip_ws_bytes(-1) == 0
     assert L.m355_grad_clip_ws_bytes(0) == L.m355_grad_clip_ws_bytes(112) == 8 * 1024 and L.m355_grad_clip_ws_bytes(113) == 2 * 8 * 1024
+
+
+def test_networks_take_group_norm(pkg):
+    """construction, parameter names and refusals of the norm switches (no GPU: nothing runs)"""
+    import argparse
+    import importlib
+    gan = importlib.import_module("2dimageto3dmodel_amd.gan")
+    rec = importlib.import_module("2dimageto3dmodel_amd.reconstruction")
+    kw = dict(conditional_class=True, conditional_color=False, conditional_text=False, n_classes=[5], texture_resolution=128, mask_output=True,
+              num_discriminators=2, texture_only=False, text_embedding_dim=256)
+    args = argparse.Namespace(norm_g="group", norm_d="group", **kw)
+    G, D = gan.Generator(args, 64), gan.MultiScaleDiscriminator(args, 4)
+    assert isinstance(G.blk1.norm1.norm, pkg.GroupNorm2d) and G.blk6.norm2.norm.num_groups == 32
+    inst = gan.MultiScaleDiscriminator(argparse.Namespace(norm_g="batch", norm_d="instance", **kw), 4)
+    assert list(D.state_dict()) == list(inst.state_dict())          # instance norm's names: weight, bias
+    with pytest.raises(ValueError):
+        gan.Generator(argparse.Namespace(norm_g="group", norm_d="none", norm_groups=48, **kw), 64)
+    a, b = rec.ReconstructionNetwork(norm="group", norm_groups=16), rec.ReconstructionNetwork()
+    assert [k for k, _ in a.named_parameters()] == [k for k, _ in b.named_parameters()]
+    assert a.bn1e.num_groups == 16 and not [k for k in a.state_dict() if "running" in k]
+    with pytest.raises(ValueError):
+        rec.ReconstructionNetwork(norm="layer")
