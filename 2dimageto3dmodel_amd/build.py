@@ -18,10 +18,10 @@ LIB = os.path.join(LIBDIR, os.environ.get("M355_BUILD_LIB", "libm355.so"))  # A/
 ARCH = "gfx950"
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-fno-fast-math", "-Wall", "-Wno-unused-function"] + os.environ.get("M355_BUILD_DEFS", "").split()
+# no packed 32-bit float instructions in any kernel: some of their forms have given wrong results on this hardware now and then.  The
+# step's time does not change (2541 / 2538 samples/s with and without them).  (hipcc's host pass does not know the feature: a harmless warning)
+DEVICE = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 STRICT = ["-ffp-contract=off"]  # bit-exactness with torch-CPU elementwise arithmetic
-
-# no packed 32-bit float instructions (the host pass of hipcc does not know the feature: its warning is harmless)
-NO_PK = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 SOURCES = [
     ("error.cpp", []),
@@ -39,11 +39,11 @@ SOURCES = [
     ("gan_glue.hip", []),
     ("gan_io.hip", []),
     ("ipc_exchange.hip", []),
-    ("group_norm.hip", NO_PK),
-    ("group_norm_f32.hip", NO_PK),
-    ("group_norm_f16.hip", NO_PK),
-    ("group_norm_bf16.hip", NO_PK),
-    ("grad_clip.hip", NO_PK),
+    ("group_norm.hip", []),
+    ("group_norm_f32.hip", []),
+    ("group_norm_f16.hip", []),
+    ("group_norm_bf16.hip", []),
+    ("grad_clip.hip", []),
     ("mesh_deform.hip", STRICT),
     ("dibr_raster.hip", STRICT),
 ]
@@ -98,7 +98,7 @@ def build(force=False, verbose=True, exact=False):
         obj = os.path.join(OBJ, name.rsplit(".", 1)[0] + ".o")
         objs.append(obj)
         if force or _newer(src, obj, headers):
-            cmd = [cc, f"--offload-arch={ARCH}", "-c", src, "-o", obj] + COMMON + extra
+            cmd = [cc, f"--offload-arch={ARCH}", "-c", src, "-o", obj] + COMMON + DEVICE + extra
             if name.endswith(".cpp"):
                 cmd = [cc, "-c", src, "-o", obj] + COMMON + extra
             if verbose:

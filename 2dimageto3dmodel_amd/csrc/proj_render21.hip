@@ -118,7 +118,7 @@ __device__ __forceinline__ Corner corner_weights(float c0, float c1, float c2, f
 }
 
 // out[k] = sum_t tap[t] * w[k + t + (kHalo - HALF)]   (FLIP: w[k - t + HALF + kHalo], the transposed convolution) for the D
-// depths of a lane from its register window, two depths per v_pk_fma_f32.  Per output the taps are accumulated in ascending
+// depths of a lane from its register window, two depths a step.  Per output the taps are accumulated in ascending
 // order with one fused multiply-add each -- the bits of the scalar loop this replaces.  The taps come from LDS (`taps`: a
 // per-lane pointer the compiler cannot prove uniform, see k_render21): one broadcast ds_read_b32 per tap.
 typedef float f2r __attribute__((ext_vector_type(2)));
