@@ -109,7 +109,7 @@ struct Place {   // what a workgroup and a thread of it own
     long long i0, ni;                   // items
     __device__ __forceinline__ Place(const Args &a, unsigned id, int V)
     {
-        const unsigned r = a.by_nblk.of(id);   // (below 2^23: the host's launches)
+        const unsigned r = a.by_nblk.of(id);   // (below 2^31: the host's launches)
         blk = (int)(id - r * (unsigned)a.nblk);
         n = (int)a.by_nslab.of(r);
         slab = (int)r - n * a.nslab;
@@ -775,20 +775,24 @@ template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds
     });
 }
 
-// ---- dw / db from cpart: row r of the result (r = sample, or the one row) adds `rows` partial rows
-static __global__ __launch_bounds__(1024) void k_gn_affine_grad(const float *__restrict__ cpart, float *__restrict__ dw, float *__restrict__ db,
-                                                                int C, long long rows)
+// ---- dw / db from cpart: row blockIdx.y of the result (a sample, or the one row) adds `rows` partial rows `gap` apart; `all` rows lie
+// between two results' first ones.  With `chunk` < rows a workgroup adds rows [z chunk, (z + 1) chunk) and leaves the sum in the first of
+// them, which no other one reads
+static __global__ __launch_bounds__(1024) void k_gn_affine_grad(float *cpart, float *dw, float *db, int C, long long all, long long rows,
+                                                                long long gap, long long chunk)
 {
     __shared__ float s1[32][33], s2[32][33];
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + cl;
-    const size_t r0 = (size_t)blockIdx.y * rows;
+    const bool part = chunk < rows;
+    const long long z0 = (long long)blockIdx.z * chunk, end = min(rows, z0 + chunk);
+    float *from = cpart + (size_t)blockIdx.y * all * 2 * C;
     float t1 = 0.0f, t2 = 0.0f;
     if (c < C) {
 #pragma unroll 4
-        for (long long r = rl; r < rows; r += 32) {
-            t1 += cpart[(r0 + r) * 2 * C + c];
-            t2 += cpart[((r0 + r) * 2 + 1) * C + c];
+        for (long long r = z0 + rl; r < end; r += 32) {
+            t1 += from[r * gap * 2 * C + c];
+            t2 += from[(r * gap * 2 + 1) * C + c];
         }
     }
     s1[rl][cl] = t1;
@@ -802,8 +806,10 @@ static __global__ __launch_bounds__(1024) void k_gn_affine_grad(const float *__r
         __syncthreads();
     }
     if (rl == 0 && c < C) {
-        if (db) db[(size_t)blockIdx.y * C + c] = s1[0][cl];
-        if (dw) dw[(size_t)blockIdx.y * C + c] = s2[0][cl];
+        float *o1 = part ? from + z0 * gap * 2 * C : db ? db + (size_t)blockIdx.y * C : nullptr;
+        float *o2 = part ? from + (z0 * gap * 2 + 1) * C : dw ? dw + (size_t)blockIdx.y * C : nullptr;
+        if (o1) o1[c] = s1[0][cl];
+        if (o2) o2[c] = s2[0][cl];
     }
 }
 

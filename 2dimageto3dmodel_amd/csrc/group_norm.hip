@@ -96,12 +96,17 @@ static long long most_rows(long long HW, int C)
     return std::max(1LL, std::min(std::max(HW, 1LL), std::min(kMostRanges, (long long)((double)HW * C / kLeast) + 2)));
 }
 
+constexpr long long kMany = 1024;   // workgroups that fill the card
+
 // One pass: slabs of whole groups whose rows are `row` bytes, if a workgroup holds one with R vectors a thread
 static bool hold(Args &a, int V, int esize, int row, int R, Choice &c)
 {
     const long long unit = unit_of(a.D, V);
     long long SC = unit;
     while (SC * esize < row && SC < a.C) SC += unit;
+    // samples of a few pixels: wider while no thread has more than one vector and workgroups abound (2048 x 512, one pixel, forward and
+    // backward: 115 -> 30 us; the slab's few threads are waited for eight times less often)
+    while (2 * SC <= a.C && a.items * (a.quad ? 4 : 1) * (2 * SC / V) <= kT && (long long)a.N * (a.C / (2 * SC)) >= kMany) SC *= 2;
     if (SC > (long long)kT * V) return false;
     set_slab(a, SC, V);
     c.R = R;
@@ -112,7 +117,7 @@ static bool hold(Args &a, int V, int esize, int row, int R, Choice &c)
 // backward of 16x16x1024 bf16 with a half-resolution residual: one sample 6.5 / 13.2 us with 64-byte rows of 4 vectors, 9.5 / 18.4 with
 // 128-byte rows of 8 (9.8 / 24.7 in two passes); 64 samples 24.3 / 75.6 and 18.9 / 48.7 (22.8 / 71.3).  8x4x512, 16 samples: 6.0 / 12.6,
 // two passes 9.4 / 23.0
-static bool one_pass(Args &a, const m355_gn_desc *d, int V, int esize, Choice &c)
+static bool one_pass(Args &a, int V, int esize, Choice &c)
 {
     if (hold(a, V, esize, 128, 4, c)) return true;
     if (hold(a, V, esize, 64, 4, c) && (long long)a.N * a.nslab <= 1024) return true;
@@ -137,10 +142,10 @@ static int check_desc(const m355_gn_desc *d)
 
 static Runner runner(int dtype) { return dtype == M355_F32 ? run_f32() : dtype == M355_F16 ? run_f16() : run_bf16(); }
 
-// f(args of these samples) over launches of at most 2^22 workgroups
+// f(args of these samples) over launches of at most 2^22 workgroups (of the kernels that give a group a wave, too)
 template <typename F> static void by_samples(const Args &all, int esize, F f)
 {
-    const long long per = std::max(1LL, (1LL << 22) / ((long long)all.nslab * all.nblk));
+    const long long per = std::max(1LL, (1LL << 22) / std::max((long long)all.nslab * all.nblk, ((long long)all.G + kT / 64 - 1) / (kT / 64)));
     for (long long n0 = 0; n0 < all.N; n0 += per) {
         Args a = all;
         a.N = (int)std::min(per, all.N - n0);
@@ -172,15 +177,24 @@ static bool past_cache(const m355_gn_desc *d, int bytes) { return (double)d->N *
 
 static unsigned wave_grid(const Args &a) { return (unsigned)(((long long)a.N * a.G + kT / 64 - 1) / (kT / 64)); }
 
+// More than kRows rows of partial sums are added in two launches, kChunk rows a workgroup in the first: 65536 x 64, forward and backward,
+// 574 -> 402 us (one launch has two workgroups for its rows there); 512 to 2048 rows: the same either way
+constexpr long long kRows = 1024, kChunk = 256;
+
 static void affine_grad(const Args &a, hipStream_t s)
 {
-    const long long rows = a.per_sample ? a.gnblk : (long long)a.N * a.gnblk;
-    const int out = a.per_sample ? a.N : 1;
-    for (int n0 = 0; n0 < out; n0 += 65535) {
-        const int k = std::min(out - n0, 65535);
-        hipLaunchKernelGGL(k_gn_affine_grad, dim3((unsigned)((a.C + 31) / 32), (unsigned)k), dim3(1024), 0, s,
-                           a.cpart + (size_t)n0 * rows * 2 * a.C, a.dw ? a.dw + (size_t)n0 * a.C : nullptr,
-                           a.db ? a.db + (size_t)n0 * a.C : nullptr, a.C, rows);
+    const long long rows = a.per_sample ? a.gnblk : (long long)a.N * a.gnblk, cols = (a.C + 31) / 32;
+    const long long chunk = std::max(kChunk, (rows + 65534) / 65535), parts = rows > kRows ? (rows + chunk - 1) / chunk : 1;
+    const int out = a.per_sample ? a.N : 1, per = (int)std::max(1LL, std::min(65535LL, (1LL << 21) / (cols * parts)));
+    for (int n0 = 0; n0 < out; n0 += per) {
+        const unsigned k = (unsigned)std::min(out - n0, per);
+        float *cpart = a.cpart + (size_t)n0 * rows * 2 * a.C;
+        float *dw = a.dw ? a.dw + (size_t)n0 * a.C : nullptr, *db = a.db ? a.db + (size_t)n0 * a.C : nullptr;
+        if (parts > 1)
+            hipLaunchKernelGGL(k_gn_affine_grad, dim3((unsigned)cols, k, (unsigned)parts), dim3(1024), 0, s, cpart, dw, db, a.C, rows, rows, 1LL,
+                               chunk);
+        hipLaunchKernelGGL(k_gn_affine_grad, dim3((unsigned)cols, k), dim3(1024), 0, s, cpart, dw, db, a.C, rows, parts > 1 ? parts : rows,
+                           parts > 1 ? chunk : 1LL, parts > 1 ? parts : rows);
     }
 }
 
@@ -231,7 +245,7 @@ extern "C" int m355_group_norm_fwd(const m355_gn_desc *d, const void *x, const f
     gn::set_items(a, res_w, res_w > 0);
     gn::set_ranges(a, 1, a.items);
     a.gnblk = 1;
-    if (gn::one_pass(a, d, c.V, es, c)) {
+    if (gn::one_pass(a, c.V, es, c)) {
         gn::by_samples(a, es, [&](const gn::Args &p) { run.one(p, c, s); });
         return check_launch("group_norm_fwd");
     }
@@ -283,7 +297,7 @@ extern "C" int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const 
     gn::set_items(a, res_w, res_w > 0);   // (the same order of additions whether or not dres is wanted)
     gn::set_ranges(a, 1, a.items);
     a.gnblk = 1;
-    if (gn::one_pass(a, d, c.V, es, c)) {
+    if (gn::one_pass(a, c.V, es, c)) {
         gn::by_samples(a, es, [&](const gn::Args &p) { run.bwd_one(p, c, s); });
         if (!a.per_sample && a.cpart) gn::affine_grad(a, s);
         return check_launch("group_norm_bwd");

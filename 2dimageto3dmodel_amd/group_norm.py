@@ -7,6 +7,7 @@ m355_group_norm_*) -- the batch-independent counterpart of gan_ops' fused batch 
 `GroupNormAct2d` the layer with its own affine (norm_d='group', ReconstructionNetwork(norm='group')).  No CPU or torch fallback: CPU
 tensors raise."""
 import ctypes
+from operator import index
 
 import torch
 import torch.nn as nn
@@ -66,7 +67,7 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
         raise TypeError(f"group_norm_act: x must be float32, float16 or bfloat16, got {x.dtype}")
     if x.dim() < 2:
         raise ValueError(f"group_norm_act: x must be [N, ..., C], got {list(x.shape)}")
-    n, c, groups = x.shape[0], x.shape[-1], int(num_groups)
+    n, c, groups = x.shape[0], x.shape[-1], index(num_groups)
     if groups < 1 or c < 1 or c % groups:
         raise ValueError(f"group_norm_act: {c} channels in {num_groups} groups")
     if not float(eps) >= 0.0:
@@ -167,7 +168,7 @@ class _GroupNormAct(torch.autograd.Function):
 
 def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
     try:
-        key = (x.shape, x.dtype, x.device, int(num_groups), float(eps), act, float(slope), w_off, out_slope, _key(weight), _key(bias),
+        key = (x.shape, x.dtype, x.device, index(num_groups), float(eps), act, float(slope), w_off, out_slope, _key(weight), _key(bias),
                None if res is None else (res.shape, res.dtype, res.device))
         p = _PLANS.get(key)
     except (AttributeError, TypeError, ValueError):   # (not tensors, not numbers: the checks say what)
@@ -195,7 +196,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu",
 
     x [N, ..., C] float32 / float16 / bfloat16 (an NCHW tensor in torch's channels_last format is `x.permute(0, 2, 3, 1)`; other
     strides are copied); num_groups divides C; every (sample, group) is normalised by its own mean and biased variance, held in
-    float32.  weight, bias: [C], or [N, C] (conditional norms: one affine per sample; rows of a larger matrix are read in place), or None
+    float32 (a group of more channels than 256 vectors hold -- of 16 bytes, or what C and the addresses are multiples of -- is refused).
+    weight, bias: [C], or [N, C] (conditional norms: one affine per sample; rows of a larger matrix are read in place), or None
     (1 / 0).  act 'lrelu': LeakyReLU(slope) -- slope 1.0 is no activation, 0.0 is ReLU, the derivative at 0 is 1 -- or 'silu'.
     res: added after the activation; x's shape, or half of x's height and width, read through the nearest x2 upsample.
     Returns y of x's shape and type, rounded once.  Gradients reach x, weight, bias and res; the results do not depend on the run."""

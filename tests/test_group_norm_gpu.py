@@ -140,6 +140,37 @@ def test_against_the_definition(pkg, shape, groups, dtype, act, slope, affine, r
     run_and_check(pkg, x, groups, w, b, r, dy, act, slope)
 
 
+@pytest.mark.parametrize("shape,groups,dtype,affine", [
+    ((2500, 48), 6, BF, "layer"),             # more partial rows than one workgroup adds, the last chunk short
+    ((2048, 1, 1, 512), 32, BF, "layer"),     # samples of one pixel: slabs wider than 128 bytes
+    ((1100, 1, 3, 320), 5, H, "sample"),      # the same, the channels no multiple of the wider slab
+    ((1500, 2, 2, 96), 3, F, "layer"),
+], ids=lambda v: str(v).replace("torch.", ""))
+def test_many_small_samples(pkg, shape, groups, dtype, affine):
+    x, w, b, _, dy = make(shape, groups, dtype, "silu", 1.0, affine, "none")
+    run_and_check(pkg, x, groups, w, b, None, dy, "silu", 1.0)
+
+
+def test_affine_gradients_of_large_samples(pkg):
+    """more ranges a sample than one workgroup adds up: per-sample dw, db against 64-bit sums of the same terms.  A chain of additions is
+    at most 64 loads of a thread, 8 lane joins, 9 rows of a chunk, 5 joins, 5 chunks and 5 joins: below K"""
+    n, h, w_, c, groups = 2, 2100, 2100, 8, 4
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(n, h, w_, c, generator=g, device=DEV).to(BF)
+    dy = (0.1 * torch.randn(n, h, w_, c, generator=g, device=DEV)).to(BF)
+    w = torch.ones(n, c, device=DEV, requires_grad=True)
+    b = torch.zeros(n, c, device=DEV, requires_grad=True)
+    dw, db = torch.autograd.grad(pkg.group_norm_act(x, groups, w, b), (w, b), dy)
+    for i in range(n):
+        xs, ds = x[i].double().reshape(-1, c), dy[i].double().reshape(-1, c)
+        xg = xs.reshape(-1, groups, c // groups)
+        rstd = ((xg - xg.mean((0, 2), keepdim=True)).pow(2).mean((0, 2), keepdim=True) + EPS).rsqrt()
+        xhat = ((xg - xg.mean((0, 2), keepdim=True)) * rstd).reshape(-1, c)
+        big = (xs.abs().amax() * rstd.max())
+        assert ((db[i] - ds.sum(0)).abs() <= K * U * ds.abs().sum(0)).all()
+        assert ((dw[i] - (ds * xhat).sum(0)).abs() <= K * U * (ds.abs() * (xhat.abs() + big)).sum(0)).all()
+
+
 @pytest.mark.parametrize("offset,outlier", [(1000.0, 0.0), (0.0, 1e4), (-30000.0, 0.0)])
 def test_statistics_do_not_cancel(pkg, offset, outlier):
     """a mean far from zero, and one far value at the place a range starts: the variance keeps its digits (bf16-exact inputs keep
@@ -180,6 +211,29 @@ def test_empty_batches(pkg):
         y.sum().backward()
         assert y.shape == x.shape and x.grad.shape == x.shape
         assert torch.equal(w.grad, torch.zeros_like(w)) and torch.equal(b.grad, torch.zeros_like(b))
+
+
+def test_refusals_on_the_device(pkg):
+    """each refused by the host, before anything is launched"""
+    x = torch.zeros(2, 6, 4, 12, device=DEV)
+    row, rows = torch.ones(12, device=DEV), torch.ones(2, 12, device=DEV)
+    f = pkg.group_norm_act
+    for bad in (lambda: f(x, 5), lambda: f(x, 0), lambda: f(x, -3), lambda: f(x[0, 0, 0], 3), lambda: f(x, 3, row[:6]), lambda: f(x, 3, rows[:1]),
+                lambda: f(x, 3, row, rows), lambda: f(x, 3, rows[:, None]), lambda: f(x, 3, eps=-1.0), lambda: f(x, 3, eps=float("nan")),
+                lambda: f(x, 3, act="gelu"), lambda: f(x, 3, res=x[:, :3]), lambda: f(x, 3, res=x[:, :3, :2, :6]),
+                lambda: f(x[:, :5], 3, res=x[:, :2, :2])):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(x.double(), 3), lambda: f(x.int(), 3), lambda: f(x, 3, row.double()), lambda: f(x, 3, None, row.int()),
+                lambda: f(x, 3, res=x.half()), lambda: f(x, 3, res=x.cpu()), lambda: f(x, 3.5), lambda: f(x, "3")):
+        with pytest.raises(TypeError):
+            bad()
+    wide = torch.zeros(2, 3, 4096, device=DEV, dtype=BF)
+    for bad in (lambda: f(x.cpu(), 3), lambda: f(x, 3, row.cpu()), lambda: f(x, 3, None, rows.cpu()), lambda: f(wide, 1),
+                lambda: f(wide[..., :257], 1)):
+        with pytest.raises(pkg._lib.M355Error):
+            bad()
+    assert torch.equal(f(x, 3, row, row), torch.ones_like(x))   # (the next call is not disturbed)
 
 
 def test_strides_and_views(pkg):
