@@ -902,6 +902,7 @@ __global__ __launch_bounds__(256) void k_dgrad_edge5(const unsigned short *__res
                 const int yy = y + kh - 2;
                 if ((unsigned)yy >= (unsigned)H) continue;
                 for (int kw = 0; kw < 5; ++kw) {
+#pragma clang fp contract(off)
                     const int xx = p + kw - 2;
                     if ((unsigned)xx >= (unsigned)W) continue;
                     const bf16x8 dv = *reinterpret_cast<const bf16x8 *>(dy + (((size_t)n * H + yy) * W + xx) * 8);

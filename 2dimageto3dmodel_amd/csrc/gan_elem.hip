@@ -321,7 +321,14 @@ __global__ __launch_bounds__(256) void k_act_bwd_apply(const act_t *__restrict__
                 const float xf = bf2f_e(vx4[u][j]);
                 const float z = xf * av[j] + bv[j];
                 const float dz = bf2f_e(vd4[u][j]) * (z >= 0.0f ? 1.0f : slope);
-                oo[j] = dz * Av[j] + xf * Bv[j] + Cv[j];
+                // (which of the products is rounded is written out, as each build always had it: the same bits from any compiler)
+#ifdef M355_EXACT
+                const float ad = dz * Av[j];
+                oo[j] = fmaf(xf, Bv[j], ad) + Cv[j];
+#else
+                const float bx = xf * Bv[j];
+                oo[j] = fmaf(dz, Av[j], bx) + Cv[j];
+#endif
             }
             *reinterpret_cast<bf16x8e *>(dx + off + (i0 + u * stride) * 8) = pack8_e(oo);
         }
@@ -401,6 +408,7 @@ __global__ __launch_bounds__(256) void k_cproj_fwd(const act_t *__restrict__ fea
     const float *e = emb + (size_t)n * C;
     float acc = 0.0f;
     for (int v = lane; v < (C >> 3); v += 64) {
+#pragma clang fp contract(off)
         const bf16x8e x = *reinterpret_cast<const bf16x8e *>(f + v * 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc += bf2f_e(x[j]) * e[v * 8 + j];

@@ -92,7 +92,8 @@ __global__ __launch_bounds__(256) void k_sn_wv(const m355_sn_layer *__restrict__
                 for (int u = 0; u < 4; ++u)
                     if (j + 64 * u < n4) {
                         const float4 a = w4[j + 64 * u], b = v4[j + 64 * u];
-                        a4[u] += (a.x * b.x + a.y * b.y) + (a.z * b.z + a.w * b.w);
+                        const float p = a.x * b.x, q = a.w * b.w;   // (each rounding written out: the same bits from any compiler)
+                        a4[u] += fmaf(a.y, b.y, p) + fmaf(a.z, b.z, q);
                     }
             }
         } else {
@@ -274,6 +275,7 @@ __global__ __launch_bounds__(1024) void k_bn_finalize(const float *__restrict__ 
         mean_o[c] = mean;
         rstd_o[c] = rstd;
         if (rmean) {
+#pragma clang fp contract(off)
             const float unb = count > 1.0f ? var * (count / (count - 1.0f)) : var;
             rmean[c] = rmean[c] * (1.0f - momentum) + mean * momentum;
             rvar[c] = rvar[c] * (1.0f - momentum) + unb * momentum;
@@ -378,6 +380,7 @@ __global__ void k_bn_bwd_coeffs(const float *__restrict__ m, float count_h, cons
                                 const float *__restrict__ mean_i, const float *__restrict__ rstd_i, int C, float *__restrict__ Bc,
                                 float *__restrict__ Cc)
 {
+#pragma clang fp contract(off)
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     if (c >= C) return;
     const float count = count_dev ? *count_dev : count_h;

@@ -451,6 +451,7 @@ __global__ __launch_bounds__(256) void k_hinge_fwd(HingeArgs a)
     const float *m = a.m[k] ? a.m[k] + (size_t)b * hw : nullptr;
     float s = 0.0f, sm = 0.0f;
     for (int i = threadIdx.x; i < hw; i += 256) {
+#pragma clang fp contract(off)
         const float mv = m ? m[i] : 1.0f;
         s += hinge_v(p[i], a.mode, real) * mv;
         sm += mv;
