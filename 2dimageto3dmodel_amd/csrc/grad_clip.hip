@@ -5,6 +5,9 @@
 // Bound: HBM (2 - 3 operations a value).  The squares are added in 64 bits -- a gradient of 1e-25 or 1e+25 has a norm, where 32-bit
 // squares give 0 or infinity -- and in a fixed order: one partial sum per workgroup, added by every workgroup of the second launch for
 // itself in the same order, so there is no third launch, no atomic and no counter to clear.
+// 24 layers of 3 x 3 x 1100 x 1100, bf16 and fp32 in turn (790 MB): squares 137 us, 5.8 TB/s, scaling 288 us, 5.5 TB/s (a copy reaches 5.4);
+// the norm alone of the bf16 list (527 MB) 84 us, 6.6 TB/s with loads past the memory-side cache.  37 tensors of 47 MB 29 us; 7 of 2 MB 10
+// us, both launches.
 // The tensors' addresses travel in the kernel arguments (kMaxT a launch): nothing is copied to the device, and a captured graph holds them.
 #include <algorithm>
 #include <math.h>

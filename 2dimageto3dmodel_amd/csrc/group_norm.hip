@@ -63,7 +63,9 @@ static bool wide_slab(Args &a, int V)
 
 constexpr long long kMostRanges = 4096;   // of a sample
 constexpr long long kLeast = 16384;       // values of a range at least
-constexpr int kJoin = 32;                 // ranges a sample up to which the second pass joins them itself
+// ranges a sample up to which the second pass joins them itself: 64 for 32 (with eight parts a lane in flight for four) saves a launch for
+// the samples between, 31.2 -> 29.0 us forward and backward of 3x100x100x96 bf16; the others stay within 1 %
+constexpr int kJoin = 64;
 
 static void set_groups(Args &a, const Choice &c)
 {

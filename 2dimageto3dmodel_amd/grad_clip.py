@@ -13,7 +13,7 @@ from . import _lib
 from ._lib import launch, lib, stream
 from .group_norm import _DTYPES, on_device
 
-_strided = torch.strided
+_strided, _same_size = torch.strided, torch.Tensor.is_same_size
 
 
 def _flat(t):
@@ -27,11 +27,12 @@ def _flat(t):
 
 
 def _check(tensors, what):
-    """-> the list, its device's index, whether every tensor's values lie together, and the lists of addresses, counts and types"""
+    """-> the list, its device's index, how every tensor's values lie (2: in order, 1: without gaps, 0: otherwise), and the lists of addresses,
+    counts and types"""
     ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not ts:
         raise ValueError(f"{what}: no gradients")
-    together, at, nums, kinds = True, [], [], []
+    together, at, nums, kinds = 2, [], [], []
     try:
         index = ts[0].get_device()
         for t in ts:
@@ -41,7 +42,7 @@ def _check(tensors, what):
             nums.append(t.numel())
             at.append(t.data_ptr())
             if together and not t.is_contiguous():
-                together = _flat(t) or t.numel() == 0
+                together = 1 if _flat(t) or t.numel() == 0 else 0
         else:
             return ts, index, together, at, nums, kinds
     except (AttributeError, KeyError, RuntimeError, NotImplementedError):   # (not tensors, or not of this kind: said below)
@@ -97,12 +98,12 @@ def clip_grads_(grads, max_norm, out=None, scale=1.0):
         raise ValueError("clip_grads_: a gradient's values have gaps or repeats between them (an expanded or sliced view)")
     outs, to = ts, at
     if out is not None:
-        outs, o_index, together, to, o_nums, o_kinds = _check(out, "clip_grads_")
+        outs, o_index, o_together, to, o_nums, o_kinds = _check(out, "clip_grads_")
         if o_index != index or o_nums != nums or o_kinds != kinds:
             raise ValueError("clip_grads_: as many outputs as gradients, of their types and shapes, on their device")
-        for t, o in zip(ts, outs):
-            if not (o.is_same_size(t) and (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride())):
-                raise ValueError("clip_grads_: an output must have its gradient's shape and strides")
+        if not (all(map(_same_size, ts, outs)) and
+                (together == o_together == 2 or all(t.is_contiguous() and o.is_contiguous() or t.stride() == o.stride() for t, o in zip(ts, outs)))):
+            raise ValueError("clip_grads_: an output must have its gradient's shape and strides")
     norm = _run(ts[0].device, index, at, to, nums, kinds, max_norm, float(scale))
     torch.autograd.graph.increment_version(outs)
     return norm

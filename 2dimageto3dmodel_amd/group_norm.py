@@ -138,32 +138,39 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stat = ctx.saved_tensors
-        p, dev = ctx.p, x.device
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        if dy.dtype != p.dtype:
-            dy = dy.to(p.dtype)
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+
+
+def _backward(ctx, dy):
+    x, weight, bias, stat = ctx.saved_tensors
+    p = ctx.p
+    need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+    if dy.dtype != p.dtype:
+        dy = dy.to(p.dtype)
+    if not dy.is_contiguous():
         dy = dy.contiguous()
-        dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(weight.shape, dtype=torch.float32, device=dev) if need_w else None
-        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if need_b else None
-        dres = dy if need_r else None
-        if need_r and p.half:
-            dres = torch.empty(p.res_shape, dtype=p.dtype, device=dev)
-        if p.empty:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif need_x or need_w or need_b or (need_r and p.half):
-            ws = torch.empty((p.ws_bwd,), dtype=torch.uint8, device=dev)
-            with on_device(p.index):
-                launch("group_norm_bwd", p.at, dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
-                       None if bias is None else bias.data_ptr(), stat.data_ptr(), None if dx is None else dx.data_ptr(),
-                       None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
-                       dres.data_ptr() if need_r and p.half else None, ws.data_ptr(), stream())
-        return dx, dw, db, dres, None
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
+    db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need_b else None
+    dres = dy if need_r else None
+    if need_r and p.half:
+        dres = torch.empty(p.res_shape, dtype=p.dtype, device=x.device)
+    if p.empty:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    elif need_x or need_w or need_b or (need_r and p.half):
+        ws = torch.empty((p.ws_bwd,), dtype=torch.uint8, device=x.device)
+        with on_device(p.index):
+            launch("group_norm_bwd", p.at, dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
+                   None if bias is None else bias.data_ptr(), stat.data_ptr(), None if dx is None else dx.data_ptr(),
+                   None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+                   dres.data_ptr() if need_r and p.half else None, ws.data_ptr(), stream())
+    return dx, dw, db, dres, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)   # (create_graph: no second derivatives)
 
 
 def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):

@@ -131,6 +131,8 @@ CASES = [
     ((257, 2, 1, 16), 2, BF, "lrelu", 0.2, "sample", "none"),   # many samples
     ((1, 300, 301, 6), 3, BF, "lrelu", 0.2, "layer", "none"),   # many ranges, the last one short
     ((1, 258, 130, 16), 2, F, "silu", 1.0, "layer", "half"),
+    ((1, 100, 100, 96), 8, BF, "lrelu", 0.2, "layer", "none"),  # 59 ranges, joined by the second pass
+    ((1, 120, 128, 64), 64, H, "silu", 1.0, "sample", "none"),  # 60 ranges, few lanes a group
 ]
 
 
