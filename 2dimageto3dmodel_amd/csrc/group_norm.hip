@@ -62,7 +62,6 @@ static bool wide_slab(Args &a, int V)
 }
 
 constexpr long long kMostRanges = 4096;   // of a sample
-constexpr long long kLeast = 16384;       // values of a range at least
 // ranges a sample up to which the second pass joins them itself: 64 for 32 (with eight parts a lane in flight for four) saves a launch for
 // the samples between, 31.2 -> 29.0 us forward and backward of 3x100x100x96 bf16; the others stay within 1 %
 constexpr int kJoin = 64;
@@ -81,21 +80,31 @@ static void set_items(Args &a, int res_w, bool quad)
     if (quad) a.by_w2.set((unsigned)a.W2);
 }
 
-// Ranges of a sample in a kernel: about total / `share` values a workgroup, within [least, most]
-static void take_ranges(Args &a, double share, long long least, long long most)
+// Values of a range: about total / few while that is within 4096 .. 16384, from there total / share up to `most`.  Small calls want
+// workgroups (5x37x29x60 fp32 forward and backward 32.1 -> 23.2 us for 16384 throughout, 2x64x32x256 bf16 25.1 -> 22.3), the first passes
+// fewer of them than the second ones, which add up what those leave (1x64x32x256 bf16 forward 10.7 us with 256 of both, 9.7); calls of
+// 4 million values lose by shorter ranges (32x32x32x128 28.8 -> 31.0)
+struct Share {
+    double few, share, most;
+    double goal(double total) const { return std::min(std::max(std::min(std::max(total / few, 4096.0), 16384.0), total / share), most); }
+};
+constexpr Share kStats = {64, 512, 131072}, kApply = {256, 1024, 32768}, kReduce = {64, 512, 32768}, kDx = {256, 1024, 32768};
+
+static void take_ranges(Args &a, const Share &sh)
 {
     const long long items = a.items;
-    const double sample = (double)a.hw * a.C, goal = std::min(std::max(sample * a.N / share, (double)least), (double)most);
-    long long nblk = (long long)(sample / a.nslab / goal + 0.999);
+    const double sample = (double)a.hw * a.C;
+    long long nblk = (long long)(sample / a.nslab / sh.goal(sample * a.N) + 0.999);
     nblk = std::max(1LL, std::min(std::min(nblk, std::max(items, 1LL)), kMostRanges));
     const long long per = std::max(1LL, (items + nblk - 1) / nblk);
     set_ranges(a, (int)std::max(1LL, (items + per - 1) / per), per);
 }
 
 // rows of partial sums a sample that any choice below may need (the workspace is sized before the pointers are known)
-static long long most_rows(long long HW, int C)
+static long long most_rows(long long N, long long HW, int C)
 {
-    return std::max(1LL, std::min(std::max(HW, 1LL), std::min(kMostRanges, (long long)((double)HW * C / kLeast) + 2)));
+    const double sample = (double)HW * C, least = std::min(kStats.goal(sample * N), kReduce.goal(sample * N));
+    return std::max(1LL, std::min(std::max(HW, 1LL), std::min(kMostRanges, (long long)(sample / least) + 2)));
 }
 
 constexpr long long kMany = 1024;   // workgroups that fill the card
@@ -208,7 +217,7 @@ using namespace m355;
 extern "C" size_t m355_group_norm_ws_bytes(const m355_gn_desc *d, int backward)
 {
     if (gn::check_desc(d) != M355_OK) return 0;
-    const size_t N = (size_t)d->N, rows = N * (size_t)gn::most_rows(d->HW, d->C);
+    const size_t N = (size_t)d->N, rows = N * (size_t)gn::most_rows(d->N, d->HW, d->C);
     size_t bytes = (rows + N) * (size_t)d->G * sizeof(float2);
     if (backward) bytes += rows * 2 * (size_t)d->C * sizeof(float);
     return (bytes + 15) / 16 * 16;
@@ -255,10 +264,10 @@ extern "C" int m355_group_norm_fwd(const m355_gn_desc *d, const void *x, const f
     gn::Args st = a;
     gn::set_items(st, 0, false);
     st.res = nullptr;
-    gn::take_ranges(st, 512, 16384, 131072);
+    gn::take_ranges(st, gn::kStats);
     st.gnblk = a.gnblk = st.nblk;
     st.gper = a.gper = st.per;
-    gn::take_ranges(a, 1024, 16384, 32768);
+    gn::take_ranges(a, gn::kApply);
     a.nt = gn::past_cache(d, es);
     a.finished = a.gnblk > gn::kJoin;
     gn::by_samples(st, es, [&](const gn::Args &p) { run.stats(p, c.V, c.A, s); });
@@ -293,7 +302,7 @@ extern "C" int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const 
     hipStream_t s = (hipStream_t)stream;
     const int es = gn::elem_bytes(dtype);
     a.gpart = (float2 *)ws;
-    a.gsum = a.gpart + (size_t)N * gn::most_rows(HW, C) * G;
+    a.gsum = a.gpart + (size_t)N * gn::most_rows(N, HW, C) * G;
     float *cpart = (float *)(a.gsum + (size_t)N * G);
     a.cpart = dw || db ? cpart : nullptr;
     gn::set_items(a, res_w, res_w > 0);   // (the same order of additions whether or not dres is wanted)
@@ -305,12 +314,12 @@ extern "C" int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const 
         return check_launch("group_norm_bwd");
     }
     gn::wide_slab(a, c.V);
-    gn::take_ranges(a, 512, 16384, 32768);
+    gn::take_ranges(a, gn::kReduce);
     a.gnblk = a.nblk;
     gn::Args p2 = a;
     gn::set_items(p2, 0, false);
     p2.dres = nullptr;
-    gn::take_ranges(p2, 1024, 16384, 32768);
+    gn::take_ranges(p2, gn::kDx);
     a.nt = p2.nt = gn::past_cache(d, 2 * es);
     a.finished = p2.finished = a.gnblk > gn::kJoin;
     gn::by_samples(a, es, [&](const gn::Args &p) { run.bwd_reduce(p, c.V, c.A, s); });

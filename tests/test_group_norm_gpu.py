@@ -131,8 +131,10 @@ CASES = [
     ((257, 2, 1, 16), 2, BF, "lrelu", 0.2, "sample", "none"),   # many samples
     ((1, 300, 301, 6), 3, BF, "lrelu", 0.2, "layer", "none"),   # many ranges, the last one short
     ((1, 258, 130, 16), 2, F, "silu", 1.0, "layer", "half"),
-    ((1, 100, 100, 96), 8, BF, "lrelu", 0.2, "layer", "none"),  # 59 ranges, joined by the second pass
-    ((1, 120, 128, 64), 64, H, "silu", 1.0, "sample", "none"),  # 60 ranges, few lanes a group
+    ((1, 100, 100, 96), 8, BF, "lrelu", 0.2, "layer", "none"),  # 64 ranges, joined by the second pass
+    ((1, 120, 128, 64), 64, H, "silu", 1.0, "sample", "none"),  # the same, few lanes a group
+    ((1, 400, 301, 24), 3, BF, "lrelu", 0.2, "layer", "full"),  # 177 ranges, joined between the passes
+    ((2, 258, 260, 32), 4, H, "silu", 1.0, "sample", "half"),
 ]
 
 
@@ -325,6 +327,48 @@ def test_same_bits_every_run_and_on_any_stream(pkg):
             torch.cuda.synchronize()
             for a, c, d in zip(want, here, other):
                 assert torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_two_threads_on_streams_of_their_own(pkg):
+    """calls of both operators from two threads at once, each on its stream: the bits of one thread alone (one-pass, joined and finished
+    statistics, shared and per-sample affines)"""
+    import threading
+    calls = []
+    for i, (shape, groups, dtype, affine, res) in enumerate([((4, 8, 4, 64), 8, BF, "sample", "none"), ((2, 64, 32, 96), 12, H, "layer", "half"),
+                                                             ((1, 400, 301, 24), 3, F, "sample", "full"), ((3, 37, 29, 60), 12, BF, "layer", "none")]):
+        x, w, b, r, dy = (None if t is None else t.to(DEV) for t in make(shape, groups, dtype, "silu", 1.0, affine, res, seed=i))
+        calls.append((x, groups, w, b, r, dy))
+
+    def work(out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(6):
+                for x, groups, w, b, r, dy in calls:
+                    leaves = [t.detach().requires_grad_() for t in (x, w, b, r) if t is not None]
+                    it = iter(leaves)
+                    xs, ws, bs, rs = (None if t is None else next(it) for t in (x, w, b, r))
+                    y = pkg.group_norm_act(xs, groups, ws, bs, act="silu", res=rs)
+                    g = torch.autograd.grad(y, leaves, dy)
+                    clipped = [t.clone() for t in g]
+                    out.append([y.detach(), *g, pkg.clip_grads_(clipped, 0.1), *clipped])
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    alone, outs, failed = [], [[], []], []
+    work(alone)
+
+    def guarded(out):
+        try:
+            work(out)
+        except Exception as e:   # (a thread's exception does not reach the test by itself)
+            failed.append(e)
+    threads = [threading.Thread(target=guarded, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for o in outs:
+        assert len(o) == len(alone) and all(torch.equal(p, q) for a, c in zip(alone, o) for p, q in zip(a, c))
 
 
 def test_captured_forward_and_backward(pkg):
