@@ -139,13 +139,13 @@ class _GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+        if torch.is_grad_enabled():   # (create_graph)
+            return _Once.apply(ctx.p, ctx.needs_input_grad, dy, *ctx.saved_tensors)
+        return _backward(ctx.p, ctx.needs_input_grad, dy, *ctx.saved_tensors)
 
 
-def _backward(ctx, dy):
-    x, weight, bias, stat = ctx.saved_tensors
-    p = ctx.p
-    need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+def _backward(p, needs, dy, x, weight, bias, stat):
+    need_x, need_w, need_b, need_r, _ = needs
     if dy.dtype != p.dtype:
         dy = dy.to(p.dtype)
     if not dy.is_contiguous():
@@ -170,7 +170,16 @@ def _backward(ctx, dy):
     return dx, dw, db, dres, None
 
 
-_backward_once = torch.autograd.function.once_differentiable(_backward)   # (create_graph: no second derivatives)
+class _Once(torch.autograd.Function):
+    """the gradients of a backward pass that is itself recorded: whoever differentiates them -- by dy, x or the affine -- is told"""
+
+    @staticmethod
+    def forward(ctx, p, needs, dy, x, weight, bias, stat):
+        return _backward(p, needs, dy, x, weight, bias, stat)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("group_norm_act can be differentiated once: no second derivatives")
 
 
 def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
@@ -207,7 +216,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu",
     weight, bias: [C], or [N, C] (conditional norms: one affine per sample; rows of a larger matrix are read in place), or None
     (1 / 0).  act 'lrelu': LeakyReLU(slope) -- slope 1.0 is no activation, 0.0 is ReLU, the derivative at 0 is 1 -- or 'silu'.
     res: added after the activation; x's shape, or half of x's height and width, read through the nearest x2 upsample.
-    Returns y of x's shape and type, rounded once.  Gradients reach x, weight, bias and res; the results do not depend on the run."""
+    Returns y of x's shape and type, rounded once.  Gradients reach x, weight, bias and res (first
+    derivatives: differentiating them again raises); the results do not depend on the run."""
     return _apply(x, num_groups, weight, bias, eps, act, slope, res, 0.0, 1.0)
 
 

@@ -371,6 +371,22 @@ def test_two_threads_on_streams_of_their_own(pkg):
         assert len(o) == len(alone) and all(torch.equal(p, q) for a, c in zip(alone, o) for p, q in zip(a, c))
 
 
+def test_create_graph(pkg):
+    """create_graph gives the same first gradients; a second derivative -- by x, the affine or dy -- is refused, not silently zero"""
+    x, w, b, r, dy = (None if t is None else t.to(DEV) for t in make((2, 6, 4, 24), 4, F, "silu", 1.0, "layer", "half"))
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    f = (lambda: pkg.group_norm_act(x, 4, w, b, act="silu", res=r))
+    plain = torch.autograd.grad(f(), leaves, dy)
+    again = torch.autograd.grad(f(), leaves, dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(plain, again))
+    for t in again:
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            t.sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        penalty = torch.autograd.grad((f() ** 2).sum(), x, create_graph=True)[0]
+        penalty.square().sum().backward()
+
+
 def test_captured_forward_and_backward(pkg):
     """two graphs (their workspaces are their own), replayed with eager work between: every replay has the eager bits"""
     cases = []
