@@ -38,7 +38,8 @@ def on_device(index):
 
 class _Plan:
     """what a call's shapes, types, strides and constants decide: the checked descriptor and the workspace sizes"""
-    __slots__ = ("desc", "at", "index", "stat", "ws", "ws_bwd", "half", "res_shape", "floats", "cast", "empty", "dtype")
+    __slots__ = ("desc", "at", "index", "stat", "ws", "ws_bwd", "half", "res_shape", "floats", "cast", "empty", "dtype", "shape", "device",
+                 "aff_shape")
 
 
 _PLANS = {}   # by shapes, types, strides, devices and constants -- never by what the tensors hold or where they lie
@@ -58,6 +59,16 @@ def _check_affine(t, name, n, c, x):
         raise ValueError(f"group_norm_act: {name} must be [{c}] or [{n}, {c}], got {list(t.shape)}")
     if t.dtype not in _DTYPES:
         raise TypeError(f"group_norm_act: {name} must be float32, float16 or bfloat16, got {t.dtype}")
+
+
+def _rows(aff, c):
+    """floats between the rows of the affine's tensors as they lie in memory (0: one row for all samples), None: their values are not rows of
+    unit stride, as far apart in one as in the other"""
+    row = aff[0].stride(0) if aff and aff[0].dim() == 2 else 0
+    for t in aff:
+        if (t.stride(-1) != 1 and c != 1) or (t.dim() == 2 and t.stride(0) != row):
+            return None
+    return row
 
 
 def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
@@ -86,8 +97,10 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
     # rows of unit channel stride, as far apart in weight as in bias, are read in place (views of a batched GEMM's output)
     per_sample = one is not None and one.dim() == 2
     aff = [t for t in (weight, bias) if t is not None]
-    plain = all(t.stride(-1) == 1 or c == 1 for t in aff) and (not per_sample or len({t.stride(0) for t in aff}) == 1) and not p.cast
-    p.floats = aff and not plain
+    row = None if p.cast else _rows(aff, c)
+    p.floats, p.aff_shape = row is None, None if one is None else tuple(one.shape)
+    if row is None:
+        row = c if per_sample else 0
     half = False
     if res is not None:
         if not torch.is_tensor(res) or res.device != x.device or res.dtype != x.dtype:
@@ -98,9 +111,9 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
             raise ValueError(f"group_norm_act: res must have x's shape {list(x.shape)} or half its height and width, got {list(res.shape)}")
     p.empty = x.numel() == 0
     p.half, p.res_shape = half, None if res is None else tuple(res.shape)
-    p.index, p.dtype = x.device.index, x.dtype
+    p.index, p.dtype, p.shape, p.device = x.device.index, x.dtype, tuple(x.shape), x.device
     p.stat = 2 * n * groups
-    p.desc = _lib.GnDesc(n, 0 if p.empty else x.numel() // (n * c), (one.stride(0) if plain else c) if per_sample else 0, c, groups,
+    p.desc = _lib.GnDesc(n, 0 if p.empty else x.numel() // (n * c), row, c, groups,
                          _DTYPES[x.dtype], ACTS[act], x.shape[2] if half else 0, int(per_sample), float(eps), float(slope),
                          float(out_slope), float(w_off))
     p.at = ctypes.addressof(p.desc)
@@ -144,8 +157,26 @@ class _GroupNormAct(torch.autograd.Function):
         return _backward(ctx.p, ctx.needs_input_grad, dy, *ctx.saved_tensors)
 
 
+def _saved(p, x, weight, bias, stat):
+    """the saved tensors as the kernels read them, and the descriptor for them.  A saved-tensor hook -- or an assignment to .data -- may bring
+    a tensor back in another layout than the plan was made for: offloading makes a slice of a wide matrix dense"""
+    aff = [t for t in (weight, bias) if t is not None]
+    if x.shape != p.shape or x.dtype is not p.dtype or x.device != p.device or stat.dtype is not torch.float32 or stat.device != p.device \
+            or stat.numel() < p.stat or any(t.shape != p.aff_shape or t.dtype is not torch.float32 or t.device != p.device for t in aff):
+        raise RuntimeError("group_norm_act: a saved tensor has come back with another shape, type or device than it was saved with")
+    x, stat, row, desc = x.contiguous(), stat.contiguous(), _rows(aff, p.shape[-1]), p.desc
+    if row is None:
+        weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+        row = p.shape[-1] if len(p.aff_shape) == 2 else 0
+    if row != desc.aff_stride:
+        desc = _lib.GnDesc.from_buffer_copy(desc)
+        desc.aff_stride = row
+    return x, weight, bias, stat, desc
+
+
 def _backward(p, needs, dy, x, weight, bias, stat):
     need_x, need_w, need_b, need_r, _ = needs
+    x, weight, bias, stat, desc = _saved(p, x, weight, bias, stat)
     if dy.dtype != p.dtype:
         dy = dy.to(p.dtype)
     if not dy.is_contiguous():
@@ -163,7 +194,7 @@ def _backward(p, needs, dy, x, weight, bias, stat):
     elif need_x or need_w or need_b or (need_r and p.half):
         ws = torch.empty((p.ws_bwd,), dtype=torch.uint8, device=x.device)
         with on_device(p.index):
-            launch("group_norm_bwd", p.at, dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
+            launch("group_norm_bwd", ctypes.addressof(desc), dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(),
                    None if bias is None else bias.data_ptr(), stat.data_ptr(), None if dx is None else dx.data_ptr(),
                    None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
                    dres.data_ptr() if need_r and p.half else None, ws.data_ptr(), stream())

@@ -1,0 +1,127 @@
+"""CPU: what group norm and gradient clipping hand to their kernels -- layouts, addresses and refusals -- with the launch replaced by a
+recorder that reads the host memory it is given (nothing runs on a GPU)."""
+import ctypes
+import importlib
+
+import pytest
+import torch
+
+
+class Dev(torch.Tensor):
+    """host memory that passes for a device tensor"""
+    is_cuda = True
+
+
+def dev(t):
+    return t.as_subclass(Dev)
+
+
+def floats(at, n, dtype=torch.float32):
+    size = torch.empty((), dtype=dtype).element_size()
+    return torch.frombuffer(bytearray(ctypes.string_at(at, n * size)), dtype=dtype)
+
+
+class Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+@pytest.fixture
+def launches(pkg, monkeypatch):
+    """the calls group_norm.py makes: (entry point, descriptor, arguments); a recorder `on[name]` is called while the memory lives"""
+    gn = importlib.import_module("2dimageto3dmodel_amd.group_norm")
+    seen, on = [], {}
+
+    def launch(name, at, *args):
+        d = pkg._lib.GnDesc.from_buffer_copy(ctypes.string_at(at, ctypes.sizeof(pkg._lib.GnDesc)))
+        seen.append((name, d, args))
+        if name in on:
+            on[name](d, *args)
+    monkeypatch.setattr(gn, "launch", launch)
+    monkeypatch.setattr(gn, "stream", lambda: 0)
+    monkeypatch.setattr(gn, "on_device", lambda index: Here())
+    seen_on = type("Launches", (), dict(seen=seen, on=on))
+    gn._PLANS.clear()
+    yield seen_on
+    gn._PLANS.clear()
+
+
+def _inputs(n=3, c=64, affine="sliced"):
+    g = torch.Generator().manual_seed(1)
+    x = dev(torch.randn(n, 4, 6, c, generator=g)).requires_grad_()
+    wide = torch.randn(n, 200, generator=g)
+    if affine == "sliced":       # rows 200 floats apart, as views of one matrix product's result are
+        w, b = dev(wide[:, 5:5 + c]), dev(wide[:, 100:100 + c])
+    elif affine == "rows":
+        w, b = dev(wide[:, :c].clone()), dev(wide[:, 100:100 + c].clone())
+    else:                        # one affine for the layer
+        w, b = dev(wide[0, :c].clone()), dev(wide[1, :c].clone())
+    return x, w.requires_grad_(), b.requires_grad_()
+
+
+def _permuted(t):
+    """the same values, the first dimension innermost in memory"""
+    return t.detach().transpose(0, -1).contiguous().transpose(0, -1)
+
+
+def _spread(t):
+    """the same values, rows (or values) 3 units further apart than they need be"""
+    s = torch.zeros(t.shape[:-1] + (t.shape[-1] * 2 + 3,))
+    return s.as_subclass(Dev)[..., :t.shape[-1]].copy_(t.detach())
+
+
+@pytest.mark.parametrize("affine", ["sliced", "rows", "layer"])
+@pytest.mark.parametrize("pack", [lambda t: t.detach().clone(), _permuted, _spread], ids=["dense", "permuted", "spread"])
+@pytest.mark.parametrize("which", ["all", "weight", "bias", "x"])
+def test_the_backward_reads_saved_tensors_where_they_lie(pkg, launches, affine, pack, which):
+    """a saved-tensor hook may bring a tensor back in another layout (a copy on the host and back makes a sliced affine dense): the kernels are
+    given the values of the forward, inside the memory that holds them"""
+    x, w, b = _inputs(affine=affine)
+    n, c = x.shape[0], x.shape[-1]
+    kept = {"weight": w, "bias": b, "x": x}
+    held, checked = [], []
+
+    def hook(t):
+        hit = which == "all" or any(k == which and t.shape == v.shape and torch.equal(t.detach(), v.detach()) for k, v in kept.items())
+        if t.dim() < 2 and t.numel() != c or not hit:
+            return t
+        held.append(pack(t))
+        return held[-1]
+
+    def backward(d, dy, xp, wp, bp, *rest):
+        row = d.aff_stride
+        assert row == (0 if affine == "layer" else row) and (affine == "layer" or row >= c)
+        for at, want in ((wp, w), (bp, b)):
+            for i in range(n if affine != "layer" else 1):
+                first = at + 4 * i * row
+                # the row lies inside some tensor that is alive: what the hook returned, what the test holds, or a copy with rows of c floats
+                inside = [t for t in held + [w, b, w._base, b._base] if t is not None
+                          and t.untyped_storage().data_ptr() <= first and first + 4 * c <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()]
+                assert inside or row == (c if affine != "layer" else 0), "a row past the memory that holds the affine"
+                assert torch.equal(floats(first, c), want.detach().as_subclass(torch.Tensor).reshape(-1, c)[i])
+        assert torch.equal(floats(xp, x.numel()), x.detach().as_subclass(torch.Tensor).reshape(-1))
+        checked.append(1)
+    launches.on["group_norm_bwd"] = backward
+    with torch.autograd.graph.saved_tensors_hooks(hook, lambda t: t):
+        y = pkg.group_norm_act(x, 8, w, b, slope=0.2)
+    assert held or which != "all"
+    torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert checked
+
+
+@pytest.mark.parametrize("change", [lambda t: t.detach()[..., :-1].clone(), lambda t: t.detach().double(), lambda t: t.detach().half(),
+                                    lambda t: t.detach().to("meta")], ids=["shape", "double", "half", "device"])
+def test_saved_tensors_that_came_back_as_others_are_refused(pkg, launches, change):
+    for which in range(4):
+        x, w, b = _inputs()
+        at = iter(range(4))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: change(t) if next(at) == which else t, lambda t: t):
+            y = pkg.group_norm_act(x, 8, w, b, slope=0.2)
+        if which == 3 and change(torch.zeros(9)).numel() < 9:
+            continue      # (the statistics' tensor may be longer than they are)
+        with pytest.raises(RuntimeError, match="saved"):
+            torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert all(name != "group_norm_bwd" for name, _, _ in launches.seen)
