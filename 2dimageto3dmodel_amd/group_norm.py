@@ -7,6 +7,7 @@ m355_group_norm_*) -- the batch-independent counterpart of gan_ops' fused batch 
 `GroupNormAct2d` the layer with its own affine (norm_d='group', ReconstructionNetwork(norm='group')).  No CPU or torch fallback: CPU
 tensors raise."""
 import ctypes
+from math import gcd
 from operator import index
 
 import torch
@@ -39,7 +40,7 @@ def on_device(index):
 class _Plan:
     """what a call's shapes, types, strides and constants decide: the checked descriptor and the workspace sizes"""
     __slots__ = ("desc", "at", "index", "stat", "ws", "ws_bwd", "half", "res_shape", "floats", "cast", "empty", "dtype", "shape", "device",
-                 "aff_shape")
+                 "aff_shape", "grid")
 
 
 _PLANS = {}   # by shapes, types, strides, devices and constants -- never by what the tensors hold or where they lie
@@ -69,6 +70,21 @@ def _rows(aff, c):
         if (t.stride(-1) != 1 and c != 1) or (t.dim() == 2 and t.stride(0) != row):
             return None
     return row
+
+
+def _grid(c, groups, size):
+    """bytes that the addresses of x, res and dy must be multiples of.  The kernels' vectors are at most 16 bytes, and what the channel count and
+    every address are multiples of; a workgroup holds a group of at most 256 vectors (segments of them where vectors straddle groups).  0: no
+    address is refused"""
+    v = 1
+    while v < 16 // size and c % (2 * v) == 0 and (c // groups) // gcd(v, c // groups) > 256:
+        v *= 2
+    return v * size if v > 1 else 0
+
+
+def _on_grid(t, grid):
+    """t, copied to an allocation of its own if a group of it were too wide from where it lies"""
+    return t.clone() if t.data_ptr() % grid else t
 
 
 def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
@@ -113,6 +129,7 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
     p.half, p.res_shape = half, None if res is None else tuple(res.shape)
     p.index, p.dtype, p.shape, p.device = x.device.index, x.dtype, tuple(x.shape), x.device
     p.stat = 2 * n * groups
+    p.grid = _grid(c, groups, x.element_size())
     p.desc = _lib.GnDesc(n, 0 if p.empty else x.numel() // (n * c), row, c, groups,
                          _DTYPES[x.dtype], ACTS[act], x.shape[2] if half else 0, int(per_sample), float(eps), float(slope),
                          float(out_slope), float(w_off))
@@ -185,6 +202,8 @@ def _backward(p, needs, dy, x, weight, bias, stat):
     dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
     db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need_b else None
     dres = dy if need_r else None
+    if p.grid:
+        x, dy = _on_grid(x, p.grid), _on_grid(dy, p.grid)
     if need_r and p.half:
         dres = torch.empty(p.res_shape, dtype=p.dtype, device=x.device)
     if p.empty:
@@ -232,6 +251,8 @@ def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
         x = x.contiguous()
     if res is not None and not res.is_contiguous():
         res = res.contiguous()
+    if p.grid:
+        x, res = _on_grid(x, p.grid), None if res is None else _on_grid(res, p.grid)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad) or (res is not None and res.requires_grad)):
         return _GroupNormAct.apply(x, weight, bias, res, p)
@@ -243,7 +264,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu",
 
     x [N, ..., C] float32 / float16 / bfloat16 (an NCHW tensor in torch's channels_last format is `x.permute(0, 2, 3, 1)`; other
     strides are copied); num_groups divides C; every (sample, group) is normalised by its own mean and biased variance, held in
-    float32 (a group of more channels than 256 vectors hold -- of 16 bytes, or what C and the addresses are multiples of -- is refused).
+    float32 (a group of more channels than 256 vectors hold -- of 16 bytes, or the widest that C is a multiple of -- is refused).
     weight, bias: [C], or [N, C] (conditional norms: one affine per sample; rows of a larger matrix are read in place), or None
     (1 / 0).  act 'lrelu': LeakyReLU(slope) -- slope 1.0 is no activation, 0.0 is ReLU, the derivative at 0 is 1 -- or 'silu'.
     res: added after the activation; x's shape, or half of x's height and width, read through the nearest x2 upsample.

@@ -125,3 +125,53 @@ def test_saved_tensors_that_came_back_as_others_are_refused(pkg, launches, chang
         with pytest.raises(RuntimeError, match="saved"):
             torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
     assert all(name != "group_norm_bwd" for name, _, _ in launches.seen)
+
+
+def _at(t, off, unit=8):
+    """the same values `off` elements behind an address that is a multiple of 64"""
+    s = torch.zeros(t.numel() + 64, dtype=t.dtype)
+    first = (-s.data_ptr() // s.element_size()) % 32 + off
+    return s.as_subclass(Dev)[first:first + t.numel()].view(t.shape).copy_(t)
+
+
+def _takes(launches):
+    """the width of a group that a workgroup holds, from the addresses: what the C entry points ask for"""
+    def accepted(d, *at):
+        size = 4 if d.dtype == 0 else 2
+        v = 16 // size
+        while v > 1 and (d.C % v or any(a % (v * size) for a in at if a)):
+            v //= 2
+        width, a, b = d.C // d.G, d.C // d.G, v
+        while b:
+            a, b = b, a % b
+        return width // a <= 256
+
+    def fwd(d, x, w, b, res, y, *rest):
+        assert accepted(d, x, res, y)
+
+    def bwd(d, dy, x, w, b, stat, dx, dw, db, dres, *rest):
+        assert accepted(d, dy, x, dx, dres)
+    launches.on.update(group_norm_fwd=fwd, group_norm_bwd=bwd)
+
+
+@pytest.mark.parametrize("c,groups,dtype", [(512, 1, torch.bfloat16), (1024, 2, torch.float16), (640, 2, torch.bfloat16), (1020, 2, torch.bfloat16),
+                                            (2048, 1, torch.float16), (1024, 1, torch.float32), (256, 1, torch.bfloat16)])
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_wide_groups_do_not_depend_on_addresses(pkg, launches, c, groups, dtype, off):
+    """a group that is taken from one address is taken from every address of an element, forward and backward"""
+    _takes(launches)
+    for which in ("x", "dy", "res", "all"):
+        x, dy, res = (dev(torch.randn(2, 4, 2, c).to(dtype)) for _ in range(3))
+        x, dy, res = (_at(t, off) if which in (k, "all") else t for k, t in (("x", x), ("dy", dy), ("res", res)))
+        x.requires_grad_()
+        res.requires_grad_()
+        y = pkg.group_norm_act(x, groups, res=res)
+        dx, dres = torch.autograd.grad(y, (x, res), dy)
+        assert torch.equal(dres, dy)
+        half = _at(torch.randn(2, 2, 1, c).to(dtype), off).requires_grad_()
+        torch.autograd.grad(pkg.group_norm_act(x, groups, res=half), (x, half), dy)
+    assert len(launches.seen) == 16
+    # a tensor that need not be copied is read in place
+    plain = [(d, a) for name, d, a in launches.seen if name == "group_norm_fwd"]
+    if off == 0 or c // groups <= 256:
+        assert plain[-1][1][0] == x.data_ptr()

@@ -42,3 +42,29 @@ def test_saved_tensors_that_were_moved(pkg, shape, groups, affine):
                 hooks(lambda t: t.transpose(0, -1).contiguous().transpose(0, -1), lambda t: t)):
         for a, k in zip(go(ctx), want):
             assert torch.equal(a, k)
+
+
+def _off_grid(t, off):
+    s = torch.empty(t.numel() + off, dtype=t.dtype, device=t.device)
+    return s[off:].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("c,groups,dtype", [(512, 1, BF), (640, 2, H), (1020, 2, BF), (1024, 1, F), (2048, 1, H)], ids=str)
+@pytest.mark.parametrize("hw", [(4, 2), (40, 64)], ids=str)
+def test_wide_groups_off_the_vector_grid(pkg, c, groups, dtype, hw):
+    """x, the residual and the incoming gradient one element behind a vector's address, one at a time and together: taken as from an aligned
+    one, with the same bits"""
+    g = torch.Generator(device=DEV).manual_seed(c)
+    x, res, dy = (torch.randn(3, *hw, c, generator=g, device=DEV).to(dtype) for _ in range(3))
+    half = torch.randn(3, hw[0] // 2, hw[1] // 2, c, generator=g, device=DEV).to(dtype)
+    w, b = 1 + 0.3 * torch.randn(c, generator=g, device=DEV), 0.2 * torch.randn(c, generator=g, device=DEV)
+
+    def go(x, res, dy):
+        ts = [t.detach().requires_grad_() for t in (x, w, b, res)]
+        y = pkg.group_norm_act(ts[0], groups, ts[1], ts[2], slope=0.2, res=ts[3])
+        return [y.detach()] + list(torch.autograd.grad(y, ts, dy))
+    for r in (res, half):
+        want = go(x, r, dy)
+        for mask in range(1, 8):
+            got = go(*(_off_grid(t, 1) if mask >> i & 1 else t for i, t in enumerate((x, r, dy))))
+            assert all(torch.equal(a, k) for a, k in zip(got, want)), mask
