@@ -11,6 +11,7 @@ from math import gcd
 from operator import index
 
 import torch
+import torch.autograd.forward_ad as fwad
 import torch.nn as nn
 
 from . import _lib
@@ -232,7 +233,14 @@ class _Once(torch.autograd.Function):
         raise RuntimeError("group_norm_act can be differentiated once: no second derivatives")
 
 
+def _has_tangent(t):
+    return torch.is_tensor(t) and fwad.unpack_dual(t).tangent is not None
+
+
 def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
+    # (a tensor with a tangent need not require a gradient: it would take the way without autograd, and lose it)
+    if fwad._current_level >= 0 and any(map(_has_tangent, (x, weight, bias, res))):
+        raise RuntimeError("group_norm_act has no forward-mode derivative")
     try:
         key = (x.shape, x.dtype, x.device, index(num_groups), float(eps), act, float(slope), w_off, out_slope, _key(weight), _key(bias),
                None if res is None else (res.shape, res.dtype, res.device))
@@ -269,7 +277,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu",
     (1 / 0).  act 'lrelu': LeakyReLU(slope) -- slope 1.0 is no activation, 0.0 is ReLU, the derivative at 0 is 1 -- or 'silu'.
     res: added after the activation; x's shape, or half of x's height and width, read through the nearest x2 upsample.
     Returns y of x's shape and type, rounded once.  Gradients reach x, weight, bias and res (first
-    derivatives: differentiating them again raises); the results do not depend on the run."""
+    derivatives: differentiating them again raises, as do forward-mode tangents); the results do not depend on the run."""
     return _apply(x, num_groups, weight, bias, eps, act, slope, res, 0.0, 1.0)
 
 

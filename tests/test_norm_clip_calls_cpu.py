@@ -175,3 +175,24 @@ def test_wide_groups_do_not_depend_on_addresses(pkg, launches, c, groups, dtype,
     plain = [(d, a) for name, d, a in launches.seen if name == "group_norm_fwd"]
     if off == 0 or c // groups <= 256:
         assert plain[-1][1][0] == x.data_ptr()
+
+
+def test_forward_mode_derivatives_are_refused(pkg, launches):
+    """a tangent is not dropped without a word: neither one of x, of the affine nor of the residual, with and without recording"""
+    import torch.autograd.forward_ad as fwad
+    for which in range(4):
+        for grad in (False, True):
+            x, w, b = (t.detach() for t in _inputs())
+            ts = [x, w, b, torch.ones_like(x)]
+            with fwad.dual_level(), torch.set_grad_enabled(grad):
+                t = ts[which].as_subclass(torch.Tensor)
+                ts[which] = dev(fwad.make_dual(t, torch.ones_like(t)))
+                assert fwad.unpack_dual(ts[which]).tangent is not None
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    pkg.group_norm_act(ts[0], 8, ts[1], ts[2], res=ts[3])
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    pkg.GroupNorm2d(64, 8)(ts[0], ts[1], ts[2], res=ts[3])
+    assert not launches.seen
+    with fwad.dual_level():      # (an open level alone changes nothing)
+        pkg.group_norm_act(x, 8)
+    assert len(launches.seen) == 1
