@@ -20,6 +20,7 @@ from ._lib import launch, lib, stream
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # m355_dtype
 ACTS = {"lrelu": 0, "silu": 1}
 _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_is_tracing = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
 
 
 class _Here:
@@ -238,6 +239,8 @@ def _has_tangent(t):
 
 
 def _apply(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slope):
+    if _is_tracing():   # (a trace records the result's allocation, not the launches; or the plan of the sizes it was made with)
+        raise RuntimeError("group_norm_act cannot be traced")
     # (a tensor with a tangent need not require a gradient: it would take the way without autograd, and lose it)
     if fwad._current_level >= 0 and any(map(_has_tangent, (x, weight, bias, res))):
         raise RuntimeError("group_norm_act has no forward-mode derivative")
@@ -277,7 +280,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="lrelu",
     (1 / 0).  act 'lrelu': LeakyReLU(slope) -- slope 1.0 is no activation, 0.0 is ReLU, the derivative at 0 is 1 -- or 'silu'.
     res: added after the activation; x's shape, or half of x's height and width, read through the nearest x2 upsample.
     Returns y of x's shape and type, rounded once.  Gradients reach x, weight, bias and res (first
-    derivatives: differentiating them again raises, as do forward-mode tangents); the results do not depend on the run."""
+    derivatives: differentiating them again raises, as do forward-mode tangents); it cannot be traced.  The results do not depend on the run."""
     return _apply(x, num_groups, weight, bias, eps, act, slope, res, 0.0, 1.0)
 
 

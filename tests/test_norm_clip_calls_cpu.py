@@ -196,3 +196,12 @@ def test_forward_mode_derivatives_are_refused(pkg, launches):
     with fwad.dual_level():      # (an open level alone changes nothing)
         pkg.group_norm_act(x, 8)
     assert len(launches.seen) == 1
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tracing_is_refused(pkg, launches, grad):
+    """a trace would record the allocation of the result and not the kernels that fill it (or, through autograd, the sizes of the first call)"""
+    ins = tuple(t.detach().as_subclass(torch.Tensor).requires_grad_(grad) for t in _inputs())
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda x, w, b: pkg.group_norm_act(dev(x), 8, dev(w), dev(b)), ins, check_trace=False)
+    assert not launches.seen
