@@ -8,10 +8,11 @@ into `out` buffers with a scale: averaging a summed message and clipping it is o
 from array import array
 
 import torch
+import torch.autograd.forward_ad as fwad
 
 from . import _lib
 from ._lib import launch, lib, stream
-from .group_norm import _DTYPES, on_device
+from .group_norm import _DTYPES, _has_tangent, _is_tracing, on_device
 
 _strided, _same_size = torch.strided, torch.Tensor.is_same_size
 
@@ -32,6 +33,10 @@ def _check(tensors, what):
     ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not ts:
         raise ValueError(f"{what}: no gradients")
+    if _is_tracing():   # (a trace records the norm's allocation, not the launches)
+        raise RuntimeError(f"{what} cannot be traced")
+    if fwad._current_level >= 0 and any(map(_has_tangent, ts)):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
     together, at, nums, kinds = 2, [], [], []
     try:
         index = ts[0].get_device()
@@ -74,7 +79,8 @@ def _run(dev, index, at, out, nums, kinds, max_norm, scale):
 
 def grad_norm(grads, scale=1.0):
     """The 2-norm of all values of `grads` (a tensor or an iterable of tensors, float32 / float16 / bfloat16 mixed, one device), times
-    |scale|: a 0-dimensional float32 tensor on their device.  Squares are added in 64 bits in a fixed order."""
+    |scale|: a 0-dimensional float32 tensor on their device.  Squares are added in 64 bits in a fixed order.  A measurement: no gradient
+    flows back through it."""
     ts, index, together, at, nums, kinds = _check(grads, "grad_norm")
     if not together:
         with torch.no_grad():

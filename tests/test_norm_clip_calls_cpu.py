@@ -205,3 +205,13 @@ def test_tracing_is_refused(pkg, launches, grad):
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda x, w, b: pkg.group_norm_act(dev(x), 8, dev(w), dev(b)), ins, check_trace=False)
     assert not launches.seen
+
+
+def test_the_norm_and_clipping_refuse_tracing_and_tangents(pkg):
+    """as group norm: a trace would hold no launch, and a tangent would be lost"""
+    import torch.autograd.forward_ad as fwad
+    for f in (lambda t: pkg.grad_norm([t, t + 1]), lambda t: pkg.clip_grads_([t], 1.0), lambda t: pkg.clip_grads_([t], 1.0, out=[t + 1])):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda x: f(dev(x)), (torch.ones(5),), check_trace=False)
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(dev(fwad.make_dual(torch.ones(5), torch.ones(5))))
