@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kT) void k_grad_scale(const Table t, const double *
     const double v = norm_of(part, nparts, scale, s);
     if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
     // (a NaN norm fails the comparison: every gradient becomes NaN; an infinite one makes the factor 0)
-    const double q = isinf(max_norm) ? 1.0 : max_norm / (v + 1e-6);   // (an infinite threshold never clips)
+    const double q = isinf(max_norm) && v == v ? 1.0 : max_norm / (v + 1e-6);   // (an infinite threshold clips nothing, not even an infinite norm)
     const float c = (float)(scale * (q >= 1.0 ? 1.0 : q));
     pieces_of(t, [&](int i, long long o, int n) {
         if (c == 1.0f && t.in[i] == t.out[i]) return;   // (times one in place)

@@ -94,8 +94,10 @@ def clip_grads_(grads, max_norm, out=None, scale=1.0):
     0-dimensional float32 tensor on their device.
 
     In place, or -- out: as many tensors of the same shapes, types and strides -- written there, the gradients left as they were.
-    max_norm >= 0, infinity never clips.  An infinite norm makes the finite gradients 0, a NaN makes all of them NaN (as
-    torch.nn.utils.clip_grad_norm_): the returned norm says so.  Tensors that share memory (the same gradient twice) are refused."""
+    max_norm >= 0.  A NaN makes all gradients NaN, whatever max_norm is; an infinite value makes the finite ones 0 (both as
+    torch.nn.utils.clip_grad_norm_).  An infinite max_norm clips nothing else, an infinite norm included: the returned norm says so.
+    (The factor comes from the 64-bit norm: one past float32's range is returned as infinity and still clips.)
+    Tensors that share memory (the same gradient twice) are refused."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads_: max_norm={max_norm!r}")

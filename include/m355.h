@@ -585,8 +585,10 @@ int m355_group_norm_bwd(const m355_gn_desc *d, const void *dy, const void *x, co
 /* ---- Global norm of a list of gradients, and clipping by it.  in / out / numel / dtype: HOST arrays of n entries (device pointers,
  *      element counts, m355_dtype).  norm (device, 1 float) = |scale| sqrt(sum of squares, added in 64 bits in a fixed order);
  *      out (nullable: the norm alone): out[i] = in[i] * scale * min(1, max_norm / (norm + 1e-6)), out[i] == in[i] allowed, any other
- *      overlap of an output with an output or with another input is M355_ERR_BAD_ARG.  max_norm infinite: never clips.  A norm that is
- *      not finite is not hidden: infinite makes the factor 0, NaN makes every output NaN.  ws >= m355_grad_clip_ws_bytes(n). */
+ *      overlap of an output with an output or with another input is M355_ERR_BAD_ARG.  A norm that is not finite is not hidden: NaN makes
+ *      every output NaN, whatever max_norm is; infinite makes the factor 0, unless max_norm is infinite, which clips nothing else.  The
+ *      factor is taken from the 64-bit norm, rounded to 32 bits: a norm past 3.4e38 is returned as infinity and still clips.
+ *      ws >= m355_grad_clip_ws_bytes(n). */
 size_t m355_grad_clip_ws_bytes(int n);
 int m355_grad_clip(const void *const *in, void *const *out, const long long *numel, const int *dtype, int n, double scale, double max_norm,
                    float *norm, void *ws, void *stream);

@@ -68,3 +68,30 @@ def test_wide_groups_off_the_vector_grid(pkg, c, groups, dtype, hw):
         for mask in range(1, 8):
             got = go(*(_off_grid(t, 1) if mask >> i & 1 else t for i, t in enumerate((x, r, dy))))
             assert all(torch.equal(a, k) for a, k in zip(got, want)), mask
+
+
+@pytest.mark.parametrize("limit", [0.0, 1.0, float("inf")])
+@pytest.mark.parametrize("form", ["in_place", "out"])
+def test_a_nan_makes_every_gradient_nan(pkg, limit, form):
+    """whatever the threshold, as torch.nn.utils.clip_grad_norm_; an infinite norm under an infinite threshold clips nothing"""
+    for bad in (float("nan"), float("inf")):
+        ts = [torch.ones(5000, device=DEV), torch.ones(77, dtype=BF, device=DEV), torch.ones(3, dtype=H, device=DEV)]
+        ts[1][5] = bad
+        out = None if form == "in_place" else [torch.zeros_like(t) for t in ts]
+        before = [t.clone() for t in ts]
+        n = pkg.clip_grads_(ts, limit, out=out)
+        got = ts if out is None else out
+        if bad != bad:
+            assert torch.isnan(n) and all(torch.isnan(t).all() for t in got)
+        elif limit == float("inf"):
+            assert torch.isinf(n) and all(torch.equal(t, b) for t, b in zip(got, before))
+        else:
+            assert torch.isinf(n) and torch.isnan(got[1][5]) and float(got[0].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0
+
+
+def test_a_norm_past_32_bits_still_clips(pkg):
+    """1000 values of 3e38: the norm, 9.5e39, is returned as infinity, the factor is the 64-bit norm's"""
+    t = torch.full((1000,), 3e38, device=DEV)
+    factor = 1e30 / float((t.double() ** 2).sum() ** 0.5 + 1e-6)
+    want = t.double() * factor
+    assert torch.isinf(pkg.clip_grads_([t], 1e30)) and ((t.double() - want).abs() <= 2.0 ** -23 * want + 2.0 ** -24 * want).all()
