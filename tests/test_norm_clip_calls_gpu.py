@@ -95,3 +95,186 @@ def test_a_norm_past_32_bits_still_clips(pkg):
     factor = 1e30 / float((t.double() ** 2).sum() ** 0.5 + 1e-6)
     want = t.double() * factor
     assert torch.isinf(pkg.clip_grads_([t], 1e30)) and ((t.double() - want).abs() <= 2.0 ** -23 * want + 2.0 ** -24 * want).all()
+
+
+def test_lists_larger_than_the_cache(pkg):
+    """from 160 MiB the kernels read and write past the memory-side cache: norm, into other buffers and in place, odd sizes and addresses, all
+    types.  Tolerances: the norm is a 64-bit sum rounded once (2^-24; 2^-23 leaves room for the sum's own 1e-12); a value is the factor's and
+    the product's 32-bit rounding and its type's"""
+    g = torch.Generator(device=DEV).manual_seed(1)
+
+    def make(n, dtype, off):
+        s = torch.empty(n + off, dtype=dtype, device=DEV)
+        return s[off:].copy_(torch.randn(n, generator=g, device=DEV))
+    ts = [make(30000001, F, 1), make(5, H, 0), make(20000003, BF, 3), make(10000019, H, 1), make(8193, F, 0), make(16384, BF, 0)]
+    before = [t.clone() for t in ts]
+    want = sum(float((t.double() ** 2).sum()) for t in ts) ** 0.5
+    limit, scale = 0.125 * want, -0.5
+    factor = scale * min(1.0, limit / (0.5 * want + 1e-6))
+    n = pkg.grad_norm(ts, scale)
+    assert abs(float(n) - 0.5 * want) <= 2.0 ** -23 * 0.5 * want
+    out = [make(t.numel(), t.dtype, 1) for t in ts]
+    assert torch.equal(pkg.clip_grads_(ts, limit, out=out, scale=scale), n)
+    assert all(torch.equal(t, b) for t, b in zip(ts, before))
+    assert torch.equal(pkg.clip_grads_(ts, limit, scale=scale), n)
+    for t, o, b in zip(ts, out, before):
+        assert torch.equal(t, o)
+        exact = b.double() * factor
+        tiny = {F: 2.0 ** -150, BF: 2.0 ** -134, H: 2.0 ** -25}[t.dtype]
+        assert ((t.double() - exact).abs() <= (torch.finfo(t.dtype).eps / 2 + 2.0 ** -23) * exact.abs() + tiny).all()
+
+
+def _check_samples(pkg, x, dy, w, b, res, groups, slope, samples):
+    """y, dx, dw, db, dres of single samples (one affine each) against the definition in 64 bits, with test_group_norm_gpu's tolerances"""
+    from test_group_norm_gpu import K, U, definition, tiny, ut
+    dtype, n, c = x.dtype, x.shape[0], x.shape[-1]
+    ts = [t.requires_grad_() for t in (x, w, b) + (() if res is None else (res,))]
+    y = pkg.group_norm_act(x, groups, w, b, slope=slope, res=res)
+    grads = torch.autograd.grad(y, ts, dy)
+    for i in samples:
+        one = [t[i:i + 1].detach().double().requires_grad_() for t in ts]
+        y6, z6, xhat, rs, big = definition(one[0], groups, one[1], one[2], "lrelu", slope, one[3] if res is not None else None)
+        d6 = dy[i:i + 1].double()
+        g6 = torch.autograd.grad(y6, one, d6.reshape(y6.shape))
+        with torch.no_grad():
+            W, D, move = one[1][:, None].abs(), d6.reshape(1, -1, c).abs(), 1 + big * rs
+            mean = (lambda t: t.reshape(1, -1, groups, c // groups).mean((1, 3), keepdim=True).expand(1, t.shape[1], groups, c // groups).reshape(t.shape))
+            r = 0.0 if res is None else one[3].repeat_interleave(2, 1).repeat_interleave(2, 2).reshape(1, -1, c).abs()
+            tol = [ut(dtype) * y6.abs() + K * U * (W * (xhat.abs() + big * rs) + one[2][:, None].abs() + r) + tiny(dtype),
+                   ut(dtype) * g6[0].reshape(1, -1, c).abs() + K * U * rs * (W * D + mean(W * D) + xhat.abs() * mean(W * D * xhat.abs())) * move + tiny(dtype),
+                   K * U * (D * (xhat.abs() + move)).sum(1), K * U * (D * move).sum(1), ut(dtype) * g6[-1].abs() + 4 * U * D.max() + tiny(dtype)]
+            got = [y[i:i + 1]] + [t[i:i + 1] for t in grads]
+            for k, (a, e) in enumerate(zip(got, [y6] + list(g6))):
+                off = (a.double().reshape(-1) - e.reshape(-1)).abs()
+                assert (off <= tol[k].reshape(-1)).all(), (i, k, float((off / tol[k].reshape(-1)).max()))
+
+
+@pytest.mark.parametrize("dtype,shape", [(BF, (5, 512, 256, 128)), (H, (9, 256, 256, 160)), (F, (5, 256, 260, 128))], ids=str)
+@pytest.mark.parametrize("half", [True, False], ids=["half", "none"])
+def test_maps_larger_than_the_cache(pkg, dtype, shape, half):
+    """160 MB and more: outputs and second reads go past the memory-side cache.  First and last sample against the definition"""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    n, h, wd, c = shape
+    x = torch.randn(shape, generator=g, device=DEV).to(dtype)
+    dy = (0.1 * torch.randn(shape, generator=g, device=DEV)).to(dtype)
+    w, b = 1 + 0.3 * torch.randn(n, c, generator=g, device=DEV), 0.2 * torch.randn(n, c, generator=g, device=DEV)
+    res = torch.randn(n, h // 2, wd // 2, c, generator=g, device=DEV).to(dtype) if half else None
+    # (no gradient arrives next to the LeakyReLU's corner)
+    from test_group_norm_gpu import definition
+    for i in (0, n - 1):
+        z = definition(x[i:i + 1].double(), 32, w[i:i + 1].double(), b[i:i + 1].double(), "lrelu", 0.2, None)[1]
+        dy[i][z.reshape(shape[1:]).abs() < 1e-3] = 0.0
+    assert x.numel() * x.element_size() >= 160e6
+    _check_samples(pkg, x, dy, w, b, res, 32, 0.2, (0, n - 1))
+
+
+@pytest.mark.parametrize("affine", ["layer", "sample"])
+def test_more_samples_than_a_launch_takes(pkg, affine):
+    """2^22 + 3 samples of one vector each: two launches.  They repeat 1021 samples, so that every value is known; the sums over the samples are
+    the repeated ones'.  A sum of dw has a chain of 9 rows of a chunk, 5 joins, 513 chunks and 5 joins: below 640"""
+    n, c, k, groups = (1 << 22) + 3, 8, 1021, 2
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x0, dy0 = torch.randn(k, c, generator=g, device=DEV).to(BF), (0.1 * torch.randn(k, c, generator=g, device=DEV)).to(BF)
+    at = torch.arange(n, device=DEV) % k
+    ws = (c,) if affine == "layer" else (k, c)
+    w0, b0 = 1 + 0.3 * torch.randn(ws, generator=g, device=DEV), 0.2 * torch.randn(ws, generator=g, device=DEV)
+
+    def go(x, w, b, dy):
+        ts = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = pkg.group_norm_act(ts[0], groups, ts[1], ts[2], act="silu")
+        return [y.detach()] + list(torch.autograd.grad(y, ts, dy))
+    few = go(x0, w0, b0, dy0)
+    many = go(x0[at], *((w0, b0) if affine == "layer" else (w0[at], b0[at])), dy0[at])
+    assert torch.equal(many[0], few[0][at]) and torch.equal(many[1], few[1][at])
+    if affine == "sample":
+        assert torch.equal(many[2], few[2][at]) and torch.equal(many[3], few[3][at])
+        return
+    one = go(x0, w0.expand(k, c), b0.expand(k, c), dy0)      # (the same sums, sample by sample)
+    for sums, total in zip(one[2:], many[2:]):
+        terms = sums.double()[at]
+        assert ((total.double() - terms.sum(0)).abs() <= 640 * 2.0 ** -24 * terms.abs().sum(0)).all()
+
+
+def test_more_samples_than_a_launch_takes_in_two_passes(pkg):
+    """2^22 + 3 samples that no workgroup's registers hold (one odd group of 129 channels, nine pixels): every launch of the two-pass form is made
+    twice, the per-sample affine's gradients in 65 parts.  They repeat 4093 samples: the same bits as those alone"""
+    n, hw, c, k = (1 << 22) + 3, 9, 129, 4093
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x0, dy0 = torch.randn(k, hw, c, generator=g, device=DEV).to(BF), (0.1 * torch.randn(k, hw, c, generator=g, device=DEV)).to(BF)
+    w0, b0 = 1 + 0.3 * torch.randn(k, c, generator=g, device=DEV), 0.2 * torch.randn(k, c, generator=g, device=DEV)
+
+    def repeat(t):
+        out = torch.empty((n,) + t.shape[1:], dtype=t.dtype, device=DEV)
+        out[:n // k * k].view((n // k,) + t.shape).copy_(t.expand((n // k,) + t.shape))
+        out[n // k * k:] = t[:n % k]
+        return out
+
+    def same(a, t):
+        return torch.equal(a[n // k * k:], t[:n % k]) and all(torch.equal(a[i * k:(i + 1) * k], t) for i in range(n // k))
+
+    def go(x, w, b, dy):
+        ts = [t.requires_grad_() for t in (x, w, b)]
+        y = pkg.group_norm_act(ts[0], 1, ts[1], ts[2], act="silu")
+        return [y.detach()] + list(torch.autograd.grad(y, ts, dy))
+    few = go(x0, w0, b0, dy0)
+    many = go(repeat(x0.detach()), repeat(w0.detach()), repeat(b0.detach()), repeat(dy0))
+    for a, t in zip(many, few):
+        assert same(a, t)
+    del many
+    torch.cuda.empty_cache()
+
+
+def test_averages_of_more_ranks_are_clipped(pkg, monkeypatch):
+    """what finish(max_norm) does with a sum over two ranks whose gradients differ: the norm and the clipped gradients are the averages'.
+    The sums are made here, as two ranks' messages would be"""
+    import importlib
+    par = importlib.import_module("2dimageto3dmodel_amd.parallel")
+    monkeypatch.setattr(par, "world_size", lambda: 2)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    shapes = ((31, 7), (5,), (64, 64, 3, 3), (1,), (200, 9))
+    for contiguous in (True, False):
+        for split in ([5], [2, 3]):
+            ranks = [[torch.randn(s, generator=g, device=DEV) for s in shapes] for _ in range(2)]
+            ps = [torch.nn.Parameter(torch.zeros(s, device=DEV)) for s in shapes]
+            for p, t in zip(ps, ranks[0]):
+                p.grad = t.clone()
+            if not contiguous:
+                ps[2].grad = ranks[0][2].permute(1, 0, 2, 3).contiguous().permute(1, 0, 2, 3)
+            parts, first = [], 0
+            for k in split:
+                mine = ps[first:first + k]
+                flat = torch.cat([(a + b).reshape(-1) for a, b in list(zip(*ranks))[first:first + k]])
+                views, at = [], 0
+                for p in mine:
+                    views.append(flat[at:at + p.numel()].view_as(p))
+                    at += p.numel()
+                parts.append((flat, mine, views))
+                first += k
+            mean = [((a + b).double() * 0.5) for a, b in zip(*ranks)]     # (the sum as the message carries it: rounded to 32 bits)
+            want = float(sum((m ** 2).sum() for m in mean)) ** 0.5
+            for limit in (0.5 * want, 2 * want):
+                keep = [f.clone() for f, _, _ in parts]
+                got = par._store_averages(parts, limit)
+                assert abs(float(got) - want) <= 2.0 ** -23 * want
+                for p, m in zip(ps, mean):
+                    exact = m * min(1.0, limit / (want + 1e-6))
+                    assert ((p.grad.double() - exact).abs() <= 2.0 ** -22 * exact.abs() + 2.0 ** -149).all()
+                for (f, _, _), t in zip(parts, keep):
+                    f.copy_(t)
+
+
+def test_networks_with_another_number_of_groups(pkg, monkeypatch):
+    """generator and discriminators with norm_groups=16 against the CPU oracle, as with the default 32"""
+    import importlib
+
+    import test_group_norm_models_gpu as models
+    lib = importlib.import_module("2dimageto3dmodel_amd._lib")
+    args, plain, seen = models._args, torch.nn.functional.group_norm, []
+    monkeypatch.setattr(models, "_args", lambda **kw: args(norm_groups=16, **kw))
+    monkeypatch.setattr(torch.nn.functional, "group_norm", lambda x, groups, *a, **kw: seen.append(groups) or plain(x, 16, *a, **kw))
+    prev = lib.set_exact(True)
+    try:
+        models.test_networks_match_the_cpu_oracle(lib)
+    finally:
+        lib.set_exact(prev)
+    assert seen
