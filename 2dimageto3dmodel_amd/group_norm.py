@@ -18,6 +18,7 @@ from . import _lib
 from ._lib import launch, lib, stream
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # m355_dtype
+_F32 = torch.float32
 ACTS = {"lrelu": 0, "silu": 1}
 _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _is_tracing = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
@@ -42,7 +43,7 @@ def on_device(index):
 class _Plan:
     """what a call's shapes, types, strides and constants decide: the checked descriptor and the workspace sizes"""
     __slots__ = ("desc", "at", "index", "stat", "ws", "ws_bwd", "half", "res_shape", "floats", "cast", "empty", "dtype", "shape", "device",
-                 "aff_shape", "grid")
+                 "aff_shape", "aff_strides", "grid")
 
 
 _PLANS = {}   # by shapes, types, strides, devices and constants -- never by what the tensors hold or where they lie
@@ -116,9 +117,10 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
     per_sample = one is not None and one.dim() == 2
     aff = [t for t in (weight, bias) if t is not None]
     row = None if p.cast else _rows(aff, c)
-    p.floats, p.aff_shape = row is None, None if one is None else tuple(one.shape)
+    p.floats, p.aff_shape = row is None, None if one is None else one.shape
     if row is None:
         row = c if per_sample else 0
+    p.aff_strides = (row, 1) if per_sample else (1,)
     half = False
     if res is not None:
         if not torch.is_tensor(res) or res.device != x.device or res.dtype != x.dtype:
@@ -129,7 +131,7 @@ def _make_plan(x, num_groups, weight, bias, eps, act, slope, res, w_off, out_slo
             raise ValueError(f"group_norm_act: res must have x's shape {list(x.shape)} or half its height and width, got {list(res.shape)}")
     p.empty = x.numel() == 0
     p.half, p.res_shape = half, None if res is None else tuple(res.shape)
-    p.index, p.dtype, p.shape, p.device = x.device.index, x.dtype, tuple(x.shape), x.device
+    p.index, p.dtype, p.shape, p.device = x.device.index, x.dtype, x.shape, x.device
     p.stat = 2 * n * groups
     p.grid = _grid(c, groups, x.element_size())
     p.desc = _lib.GnDesc(n, 0 if p.empty else x.numel() // (n * c), row, c, groups,
@@ -179,18 +181,25 @@ class _GroupNormAct(torch.autograd.Function):
 def _saved(p, x, weight, bias, stat):
     """the saved tensors as the kernels read them, and the descriptor for them.  A saved-tensor hook -- or an assignment to .data -- may bring
     a tensor back in another layout than the plan was made for: offloading makes a slice of a wide matrix dense"""
-    aff = [t for t in (weight, bias) if t is not None]
-    if x.shape != p.shape or x.dtype is not p.dtype or x.device != p.device or stat.dtype is not torch.float32 or stat.device != p.device \
-            or stat.numel() < p.stat or any(t.shape != p.aff_shape or t.dtype is not torch.float32 or t.device != p.device for t in aff):
+    dev = p.device
+    changed = x.shape != p.shape or x.dtype is not p.dtype or x.device != dev or stat.dtype is not _F32 or stat.device != dev \
+        or stat.numel() < p.stat
+    moved = False
+    for t in (weight, bias):
+        if t is not None:
+            changed = changed or t.shape != p.aff_shape or t.dtype is not _F32 or t.device != dev
+            moved = moved or t.stride() != p.aff_strides
+    if changed:
         raise RuntimeError("group_norm_act: a saved tensor has come back with another shape, type or device than it was saved with")
-    x, stat, row, desc = x.contiguous(), stat.contiguous(), _rows(aff, p.shape[-1]), p.desc
-    if row is None:
-        weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-        row = p.shape[-1] if len(p.aff_shape) == 2 else 0
-    if row != desc.aff_stride:
+    desc = p.desc
+    if moved:
+        row = _rows([t for t in (weight, bias) if t is not None], p.shape[-1])
+        if row is None:
+            weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+            row = p.shape[-1] if len(p.aff_shape) == 2 else 0
         desc = _lib.GnDesc.from_buffer_copy(desc)
         desc.aff_stride = row
-    return x, weight, bias, stat, desc
+    return x.contiguous(), weight, bias, stat.contiguous(), desc
 
 
 def _backward(p, needs, dy, x, weight, bias, stat):
