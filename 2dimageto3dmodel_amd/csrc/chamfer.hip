@@ -7,10 +7,11 @@
 //   * targets are staged as x[1024] | y[1024] | z[1024]: ONE ds_read_b128 broadcasts a coordinate of FOUR targets;
 //   * the distance arithmetic is written two targets at a time (the file is compiled with -ffp-contract=off, the two fused
 //     operations are written out): every distance has the oracle's bits, fma(dz, dz, fma(dy, dy, dx*dx)).  The library is built
-//     without packed fp32 instructions: the pairs become two scalar operations each, at the same measured rate (70 TF);
+//     without packed fp32 instructions: the pairs become two scalar operations each, at the rate the packed form had (16 pairs of
+//     clouds of 16384 points: 70.3 TF without, 70.6 with them);
 //   * the sweep only tracks the running MINIMUM (one v_min3_f32 per two pairs) and, per 64-target chunk, whether it
 //     improved; the index is recovered afterwards by re-scanning that one chunk for the first target attaining the
-//     minimum (lowest j on ties, as the oracle): 3.5 VALU + 0.19 LDS instructions per pair (round 1: 11 + 3);
+//     minimum (lowest j on ties, as the oracle): 6.5 VALU + 0.19 LDS instructions per pair (the first version: 11 + 3);
 //   * small problems (B = 1) get 16 waves per workgroup over 64 queries instead of a quarter-filled chip.
 #include <stdlib.h>
 #include "common.h"

@@ -734,7 +734,7 @@ __device__ __forceinline__ void dx_store(const Args &a, const float (&f)[V], con
     IO<T, V>::template store<NT>(dx, xc);
 }
 
-// ---- backward, second pass: dx.  Large: 125 us, 6.4 TB/s (805 MB); 16 x 64 x 32 x 256 bf16 9.9 us
+// ---- backward, second pass: dx.  Large: 126 us, 6.4 TB/s (805 MB); 16 x 64 x 32 x 256 bf16 9.9 us
 template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds__(kT) void k_gn_bwd_apply(const Args a)
 {
     typedef typename IO<T, V>::raw raw;
@@ -783,7 +783,7 @@ template <typename T, int V, int A, int ACT, bool NT> __global__ __launch_bounds
     });
 }
 
-// ---- dw / db from cpart (4 to 5 us: the launch and one way to memory): row blockIdx.y of the result (a sample, or the one row) adds `rows` partial rows `gap` apart; `all` rows lie
+// ---- dw / db from cpart (3 to 5 us: the launch and one way to memory): row blockIdx.y of the result (a sample, or the one row) adds `rows` partial rows `gap` apart; `all` rows lie
 // between two results' first ones.  With `chunk` < rows a workgroup adds rows [z chunk, (z + 1) chunk) and leaves the sum in the first of
 // them, which no other one reads
 static __global__ __launch_bounds__(1024) void k_gn_affine_grad(float *cpart, float *dw, float *db, int C, long long all, long long rows,

@@ -8,7 +8,7 @@ namespace {
 typedef M355_GN_T T;
 constexpr int kV = 16 / sizeof(T);   // the widest vector
 
-// f(V, A) of the vectors and segments that are built: pick() in group_norm.hip chooses among these
+// f(V, A) of the vectors and segments that are built: pick_vec() in group_norm.hip chooses among these
 template <typename F> void by_vector(int V, int A, F f)
 {
     using std::integral_constant;

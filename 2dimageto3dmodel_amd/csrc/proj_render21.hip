@@ -126,7 +126,7 @@ template <int NT, int D, int WIN, bool FLIP>
 __device__ __forceinline__ void depth_conv(const float (&w)[WIN], const float *taps, float (&out)[D])
 {
     constexpr int HALF = NT / 2;
-    static_assert(D % 2 == 0, "two depths per packed operation");
+    static_assert(D % 2 == 0, "two depths a step");
     f2r acc[D / 2];
 #pragma unroll
     for (int m = 0; m < D / 2; ++m) acc[m] = f2r{0.0f, 0.0f};
@@ -197,9 +197,9 @@ __global__ __launch_bounds__(kThreads21) void k_render21(Render21Args a)
         return;
     }
 
-    // The NT taps are uniform: left to the compiler they live in SGPRs, and the packed FMAs of the backward (two convolutions)
-    // want each as an SGPR PAIR -- 42 + the rest overflowed the scalar file: 40-81 SGPR spills into VGPR lanes and 160
-    // v_readlane_b32 (+ hazard nops) inside the per-ray loop (round 4, from the ISA).  They sit in LDS instead and each tap is
+    // The NT taps are uniform: left to the compiler they live in SGPRs.  Built with packed FMAs, which want each as an SGPR PAIR,
+    // the two convolutions of the backward overflowed the scalar file: 40-81 SGPR spills into VGPR lanes and 160
+    // v_readlane_b32 (+ hazard nops) inside the per-ray loop (from the ISA).  They sit in LDS instead and each tap is
     // read (one broadcast ds_read_b32) right where its D FMAs are issued.
     // DETS: the fixed-point scale of THIS tile = the largest power of two that keeps (its number of records) maximal weights inside
     // 62 bits, never finer than 2^-40.  Literal weights reach (2S)^3 in magnitude with either sign (tri:66), the "fixed" ones 1.
